@@ -108,7 +108,7 @@ __global__ __launch_bounds__(kThreads) void slx_cloud_fused_kernel(const SlxClou
     const unsigned P = (unsigned)q.parts, R = (unsigned)q.rows_per_part, n_slots = (unsigned)q.groups * P;
     double *tile = lds, *run = lds + (size_t)R * 16u + (size_t)wave * 192u;
     unsigned long long *totals = q.words + SLX_CLOUD_COUNTERS * 16u, *cols = totals + n_slots;
-    // The ticket.  ONE counter for all workgroups serialises them (a counter hands out ~88 tickets per microsecond, tools/probes/satomic.hip:
+    // The ticket.  ONE counter for all workgroups serialises them (a counter hands out ~88 tickets per microsecond:
     // 600 workgroups waited 7 us for theirs in the first version).  So the workgroups are dealt into SLX_CLOUD_COUNTERS classes by their
     // index and class c numbers its members c, c + C, c + 2 C ... in the order they start: within a class a lower ticket has started
     // earlier; across classes the dispatcher, which starts workgroups in index order, keeps the classes within one of each other, so the

@@ -1257,6 +1257,31 @@ __global__ __launch_bounds__(256) void slx_strip_kernel(const SlxKParams p)
     }
 }
 
+// A wave's view of its work queue (the stream kernels below): tickets count up from 0 within a launch.
+struct TicketQueue {
+    unsigned *ctr;
+    unsigned zero;                                 // 0 in a vector register: an address the compiler knows to be uniform would make it
+                                                   // rewrite the atomic as a wave-wide sum, read back (and waited for) on the spot
+    unsigned last;                                 // the last ticket of the launch
+    __device__ __forceinline__ TicketQueue(unsigned *counters, unsigned q, unsigned n_items, unsigned n_waves)
+        : ctr(counters + (size_t)q * 32u), last(n_items + n_waves - 1u)
+    {
+        asm volatile("v_mov_b32 %0, 0" : "=v"(zero));
+    }
+    // one relaxed add at device scope (the queue's waves sit on all XCDs); the ticket is in lane 0 of the result
+    __device__ __forceinline__ unsigned draw(unsigned lane) const
+    {
+        unsigned old = ~0u;
+        if (lane == 0) old = __hip_atomic_fetch_add(ctr + zero, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        return old;
+    }
+    // Every wave draws until its first failing ticket and nobody draws after the last one: whoever drew it resets the counter.
+    __device__ __forceinline__ void reset_behind_last(unsigned ticket, unsigned lane) const
+    {
+        if (ticket == last && lane == 0) __hip_atomic_store(ctr + zero, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+};
+
 // ------------------------------------------------------------------------------------------
 // Stream kernel (round 4): the 3 x 4-step class (Gray-free, depth only) with work handed out in ADDRESS ORDER to resident waves.
 //
@@ -1267,17 +1292,25 @@ __global__ __launch_bounds__(256) void slx_strip_kernel(const SlxKParams p)
 // LAUNCH and then takes short items (R rows of one 64-quad chunk column) from a queue until the queue is empty:
 //   * queue q = (chunk column c, residue j): its k-th item is row group G = k m + j of the batch's frame-sets laid end to end
 //     (G -> frame-set, group by one scalar multiply-high), always of column c -- so the wave's per-column state never changes;
-//   * a ticket is ONE scalar atomic (s_atomic_add ... glc: old value to an SGPR, counted by lgkmcnt, no vector register, not in
-//     the vmcnt sequence the DMA ring counts) issued just before the step's wait for its DMA chunk, so its latency hides there;
+//   * a ticket is ONE atomic add of one lane (TicketQueue above).  Its result comes back IN the vmcnt sequence that the DMA ring counts, so
+//     it is drawn a step before it is needed, directly behind the step's counted wait: L(s) retired | T Z(s-1) L(s+2) | ..., and
+//     the next step's wait for L(s+1), which leaves Z and L(s+2) in flight, retires T with it.  What T waits for in that order (L(s+1))
+//     the next step needs anyway, so a ticket costs no look-ahead; the price is one item more in hand (A, B, and at A's last row the
+//     item after B);
 //   * the queues' fronts advance together: at any moment the resident waves hold a band of consecutive row groups of one or two
 //     frame-sets, whatever the speed of the single waves (oldest-first arbitration makes them unequal: a slow wave simply takes
 //     fewer items) -- the footprint of short items with the start-up cost of one item per wave;
 //   * the DMA ring (two chunks ahead), the counted waits, the staged lane-contiguous stores are the strip kernel's, carried
-//     across item boundaries: the request side runs two rows ahead of the compute side and crosses into the next item first.
+//     across item boundaries: the request side runs two rows ahead of the compute side and crosses into the next item first;
+//   * every step issues the SAME vector-memory operations behind its wait: where a row has no predecessor to store, or the request side
+//     no item left, they go to an empty descriptor (num_records 0: nothing is read or stored).  The counted waits are
+//     then one constant, and hipcc's own wait in front of the ticket's use counts to the same operations instead of draining the ring
+//     (tests/test_kernel_resources.py walks the compiled code).
+// Same box, against the strip kernel: C4 x 32 283.4 -> 271.7 us (5.43 TB/s of planes in and depth out), x 8 80.3 -> 74.1, C2 x 80 287.9 -> 269.9.
 // Counters: one 32-bit word per queue, 128 bytes apart (p.sq_counters); a launch draws exactly K_q + W_q tickets from counter q (K_q
-// items, one failing ticket per wave), and the wave that draws the last one puts the counter back to zero (round 6; rounds 4-5 let
-// the counters run on and told the kernel the launch's number): every launch starts from zero, the host zeroes the words once when
-// it allocates them and after a failed launch, and a captured launch can be replayed.
+// items, one failing ticket per wave: a wave draws only while the ticket before was good), and the wave that drew the last one puts the
+// counter back to zero when it ends: every launch starts from zero, the host zeroes the words once when it allocates them and after a
+// failed launch, and a captured launch can be replayed.
 template <int F>
 __global__ __launch_bounds__(256) void slx_stream_kernel(const SlxKParams p)
 {
@@ -1302,19 +1335,7 @@ __global__ __launch_bounds__(256) void slx_stream_kernel(const SlxKParams p)
     const unsigned c = q % cpg, j = q / cpg;
     const unsigned Kq = p.sq_groups_total > j ? (p.sq_groups_total - j + m - 1u) / m : 0u;     // items of this queue
     const unsigned Wq = (total_waves - q + NQ - 1u) / NQ;                                       // waves that poll it
-    const unsigned last_ticket = Kq + Wq - 1u;                                                  // a launch draws exactly K_q + W_q tickets from queue q
-    unsigned *ctr = p.sq_counters + (size_t)q * 32u;
-    auto fetch_issue = [&](unsigned &raw) {        // the ticket arrives with the next s_waitcnt lgkmcnt(0)
-        asm volatile("s_mov_b32 %0, 1\n\ts_atomic_add %0, %1, 0x0 glc" : "=&s"(raw) : "s"(ctr) : "memory");
-    };
-    auto fetch_wait = [&](unsigned &raw) { asm volatile("s_waitcnt lgkmcnt(0)" : "+s"(raw)::"memory"); };
-    // The wave that draws a queue's LAST ticket of the launch (every wave draws until its first failing one: K_q + W_q draws in all, and
-    // nobody draws after the last) puts the counter back to zero -- a scalar atomic without return, outside the vmcnt sequence.  Every
-    // launch therefore finds its counters at zero, whatever ran before it: nothing to reset from the host between launches or
-    // geometries, and a launch captured into a hipGraph can be replayed (rounds 4-5 kept an epoch on the host, which a replay repeats).
-    auto reset_behind_last = [&](unsigned raw) {
-        if (raw == last_ticket) asm volatile("s_atomic_and %0, %1, 0x0" ::"s"(0u), "s"(ctr) : "memory");
-    };
+    const TicketQueue queue(p.sq_counters, q, Kq, Wq);
 
     // ---- per-column state, once per launch
     const unsigned W = (unsigned)p.width, H = (unsigned)p.height;
@@ -1351,21 +1372,21 @@ __global__ __launch_bounds__(256) void slx_stream_kernel(const SlxKParams p)
 
     // ---- items: ticket -> (frame-set, first row of the row group)
     struct Item { unsigned valid, set, row_base; };
-    auto decode = [&](unsigned raw) {
+    auto decode = [&](unsigned k) {
         Item it;
-        const unsigned k = raw;
         it.valid = k < Kq ? 1u : 0u;
         const unsigned G = it.valid ? k * m + j : 0u;
         it.set = p.sq_groups_per_set == 1u ? G : __umulhi(G, p.sq_magic);   // G / groups_per_set (exact for G * groups_per_set < 2^32: slx_plan.cpp)
         it.row_base = (G - it.set * p.sq_groups_per_set) * R * il;
         return it;
     };
-    unsigned raw;
-    fetch_issue(raw);
-    fetch_wait(raw);
-    reset_behind_last(raw);
-    Item A = decode(raw), B{0u, 0u, 0u};
-    if (!A.valid) return;
+    unsigned ticket = uniform_u32(queue.draw(lane));               // the newest ticket this wave has drawn
+    Item A = decode(ticket);
+    if (!A.valid) {
+        queue.reset_behind_last(ticket, lane);
+        return;
+    }
+    const unsigned second = queue.draw(lane);                      // arrives behind the first requests
 
     // request side (two chunks ahead): its item, rows of it already requested, descriptor, lane offset of the next row to request
     Item D = A;
@@ -1377,29 +1398,20 @@ __global__ __launch_bounds__(256) void slx_stream_kernel(const SlxKParams p)
         const unsigned voff = dma_off < dma_last ? dma_off : dma_last;
         uint32_t *dst = ring + slot * ROW_DW;
         unsigned so = p.phase_first;
-        if (p.dma_imm) {
-            static_for<NPH>([&](auto k) {
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(drsrc, (lds_void *)dst, 4, voff, so, decltype(k)::value * 256, 2 /* nt */);
-                if (decltype(k)::value + 1 < NPH) next_plane(so, p.phase_step - 256u);
-            });
-        } else {
-#pragma unroll
-            for (int k = 0; k < NPH; k++) {
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(drsrc, (lds_void *)(dst + k * 64), 4, voff, so, 0, 2 /* nt */);
-                if (k + 1 < NPH) next_plane(so, p.phase_step);
-            }
-        }
+        static_for<NPH>([&](auto k) {                              // (p.dma_imm: the plan takes this kernel only where it holds)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(drsrc, (lds_void *)dst, 4, voff, so, decltype(k)::value * 256, 2 /* nt */);
+            if (decltype(k)::value + 1 < NPH) next_plane(so, p.phase_step - 256u);
+        });
         dma_off += dma_step;
         dri = uniform_u32(dri + 1u);
     };
-    // the request side steps into item `to` (its first row comes next)
+    // the request side steps into item `to` (its first row comes next); behind the last item it reads from an empty descriptor
     auto request_moves_to = [&](const Item &to) {
         D = to;
         dri = 0;
-        if (to.valid) {
-            drsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(uniform_ptr(p.plane_base + (size_t)to.set * p.phase_set_stride)), 0, 0xFFFFFFFFu, 0x00020000);
-            dma_off = dma_lane + to.row_base * row_stride;
-        }
+        drsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(uniform_ptr(p.plane_base + (size_t)to.set * p.phase_set_stride)), 0,
+                                                  uniform_u32(to.valid ? 0xFFFFFFFFu : 0u), 0x00020000);
+        dma_off = dma_lane + to.row_base * row_stride;
     };
 
     // compute side: item A, row ri of it; where its rows are stored
@@ -1407,12 +1419,21 @@ __global__ __launch_bounds__(256) void slx_stream_kernel(const SlxKParams p)
     unsigned row = A.row_base + sub;
     __amdgpu_buffer_rsrc_t zrsrc = __builtin_amdgcn_make_buffer_rsrc(p.z + (size_t)A.set * p.out_set_stride, 0, H * W * 8u, 0x00020000);
     unsigned out_boff[2] = {out_lane[0] + A.row_base * W * 8u, out_lane[1] + A.row_base * W * 8u};
-    // the staged row waiting for its (one step late) stores
-    __amdgpu_buffer_rsrc_t prsrc = zrsrc;
-    unsigned pend_off[2] = {0xFFFFFFF0u, 0xFFFFFFF0u};
-    issue_chunk(0);                                                // rows 0 and 1 of the first item (R >= 2)
+    // the staged row waiting for its (one step late) stores; none yet: an empty descriptor drops them
+    __amdgpu_buffer_rsrc_t prsrc = __builtin_amdgcn_make_buffer_rsrc(p.z, 0, 0u, 0x00020000);
+    unsigned pend_off[2] = {0u, 0u};
+    auto flush_row = [&]() {
+#pragma unroll
+        for (int k = 0; k < NZ; k++) {
+            const u32x4 v = *reinterpret_cast<const u32x4 *>(stage + k * 64 + lane);
+            __builtin_amdgcn_raw_buffer_store_b128(v, prsrc, pend_off[k], 0, 2 /* nt */);
+        }
+    };
+    issue_chunk(0);                                                // rows 0 and 1 of the first item (R >= 2), spaced like every step's
+    flush_row();
     issue_chunk(1);
-    unsigned ahead = 2;                                            // chunks requested and not yet waited for
+    ticket = uniform_u32(second);
+    Item B = decode(ticket);
     for (unsigned s = 0;; s++) {
         const unsigned slot = s & 1u;
         // Priority while a wave works towards its next DMA request (wait, flush, LDS reads, phase arithmetic, request), none in the
@@ -1420,24 +1441,13 @@ __global__ __launch_bounds__(256) void slx_stream_kernel(const SlxKParams p)
         // C4 x 32 268.8 vs 274.9 us (-2.2 %), C2 x 80 270.9 vs 275.1 (-1.5 %); priority in the tail instead: +1.7 %; priority only up
         // to an EARLIER request (all dwords first, then the request, then the arithmetic): +1 %.
         __builtin_amdgcn_s_setprio(1);
-        // The ticket of the item after this one; lands below.  A variable of this step alone: its live range is the window between its
-        // issue and its wait and nothing else (a variable carried around the loop is live everywhere, and the allocator then saves and
-        // restores its register around whatever needs scalar registers -- harmless after the wait, fatal inside the window;
-        // tests/test_kernel_resources.py pins the compiled code)
-        unsigned next_raw;
-        if (ri == 0) fetch_issue(next_raw);
-        // counted wait for chunk s (vmcnt retires in issue order): L(s) | Z(s-2) L(s+1) | wait -- as in slx_strip_kernel
-        if (ahead < 2u) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        else if (s >= 2u) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NPH + NZ) : "memory");
-        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NPH) : "memory");
-        ahead--;
-        if (s > 0) {                                               // last row's stores, one step late
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const u32x4 v = *reinterpret_cast<const u32x4 *>(stage + k * 64 + lane);
-                __builtin_amdgcn_raw_buffer_store_b128(v, prsrc, pend_off[k], 0, 2 /* nt */);
-            }
-        }
+        // counted wait for chunk s (vmcnt retires in issue order): L(s) | T(s-1) Z(s-2) L(s+1) | wait -- Z and L stay in flight
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NPH + NZ) : "memory");
+        // the ticket of the item after B, drawn at A's last row and used at the end of this step
+        const bool last_row = ri + 1u == R;
+        unsigned next = ~0u;
+        if (last_row && B.valid) next = queue.draw(lane);
+        flush_row();                                               // last row's stores, one step late
         float pix[F][SLX_QUAD];
         if (row < H) {
             const uint32_t *src = ring + slot * ROW_DW + lane;
@@ -1455,20 +1465,10 @@ __global__ __launch_bounds__(256) void slx_stream_kernel(const SlxKParams p)
                 pix[f][3] = px.b.y;
             }
         }
-        // the slot is free once it has been read -- and the ticket requested above has arrived with the same wait
-        if (ri == 0) {
-            fetch_wait(next_raw);
-            reset_behind_last(next_raw);
-            B = decode(next_raw);
-        } else {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        }
-        // chunk s + 2: the request side's next row, in this item or the first row of the next one
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");         // the slot is free once it has been read
+        // chunk s + 2: the request side's next row, in this item or the first row of the next one (or none)
         if (D.valid && dri == R) request_moves_to(B);
-        if (D.valid) {
-            issue_chunk(slot);
-            ahead++;
-        }
+        issue_chunk(slot);
         __builtin_amdgcn_s_setprio(0);
         if (row < H) {
             double z[SLX_QUAD];
@@ -1506,9 +1506,11 @@ __global__ __launch_bounds__(256) void slx_stream_kernel(const SlxKParams p)
         __builtin_amdgcn_wave_barrier();
         // next row of the item, or the next item
         ri = uniform_u32(ri + 1u);
-        if (ri == R) {
+        if (last_row) {
             if (!B.valid) break;
             A = B;
+            ticket = uniform_u32(next);
+            B = decode(ticket);
             ri = 0;
             row = A.row_base + sub;
             zrsrc = __builtin_amdgcn_make_buffer_rsrc(uniform_ptr(p.z + (size_t)A.set * p.out_set_stride), 0, H * W * 8u, 0x00020000);
@@ -1520,12 +1522,10 @@ __global__ __launch_bounds__(256) void slx_stream_kernel(const SlxKParams p)
             out_boff[1] += out_step;
         }
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-        const u32x4 v = *reinterpret_cast<const u32x4 *>(stage + k * 64 + lane);
-        __builtin_amdgcn_raw_buffer_store_b128(v, prsrc, pend_off[k], 0, 2 /* nt */);
-    }
+    // no DMA may land in LDS behind the wave's end, the empty ones of the last steps included
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    flush_row();
+    queue.reset_behind_last(ticket, lane);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -1536,16 +1536,16 @@ __global__ __launch_bounds__(256) void slx_stream_kernel(const SlxKParams p)
 // chunk column from its queue (same queues, tickets and counters).  What differs from that kernel:
 //   * a row is TWO ring chunks -- its 4 phase planes (slot 0) and its 12 Gray planes (slot 1) -- so the request side runs one row
 //     ahead: the phase chunk of row r + 1 is requested once the phase dwords of row r have been read, the Gray chunk likewise;
-//   * counted waits (vmcnt retires in issue order):  P(r) G(r) | Z(r-1) P(r+1) | G(r+1) Z(r) ...: the wait for P(r) leaves G(r) in
-//     flight (NGR), the wait for G(r) leaves Z(r-1) and P(r+1) (NZ + NPH; the launch's first row has no Z in front of it);
+//   * counted waits (vmcnt retires in issue order):  P(r) T G(r) | Z(r-1) P(r+1) | T G(r+1) | Z(r) ...: the wait for P(r) leaves G(r)
+//     in flight (NGR) and retires the ticket T with P(r); the wait for G(r) leaves Z(r-1) and P(r+1) (NZ + NPH).  T goes between the two
+//     chunks: drawn behind the wait for G(r), it is used when the row's arithmetic is done, at the end of the step;
 //   * items of ONE row (slx_plan.cpp): REF x 32 164.3 us with 1-row items, 171.3 with 2, 177.6 with 3, 192 with 8 -- the waves of a
 //     SIMD wait for their DMA here, and the more often they draw tickets the less they move in step.
-// Same-box A/B against the strip kernel (profiles/r06_gstream_ab.log): REF x 32 169.5 -> 164.3 us (-3.1 %), x 16 -3.5 %, x 8 -2.4 %, x 4
-// +0.7 %; 55.7 M vector instructions per launch for 59.9 M, the same bytes.  The Gray-MASK mode (x3: 62-quad spans with halo lanes)
+// Same-box A/B against the strip kernel: REF x 32 168.9 -> 166.1 us (-1.7 %), x 8 49.1 -> 48.1 (-2.0 %).  hipcc places the waits of the table
+// look-up (codes other than the reflected one) behind the join of both arms: the DMA in flight is drained there in either case.  55.7 M vector instructions per launch for 59.9 M, the same bytes.  The Gray-MASK mode (x3: 62-quad spans with halo lanes)
 // was built on this kernel too, in five versions -- chip-wide queues (1 282 MB read for 885 algorithmic: the two waves that share a
 // halo line almost never share an L2), XCD-local queues (1 017 MB), one ticket per workgroup and item handed over through LDS (942 MB)
-// -- and none beat the strip kernel's statically aligned items by 2 % on config 3 (best: -1.2 %): not in the tree
-// (profiles/experiments/r06_gstream_kernel_gray_mask_mode.patch).
+// -- and none beat the strip kernel's statically aligned items by 2 % on config 3 (best: -1.2 %): not in the tree.
 __global__ __launch_bounds__(256) void slx_gstream_kernel(const SlxKParams p)
 {
     constexpr int F = 1, GB = 6;
@@ -1571,15 +1571,7 @@ __global__ __launch_bounds__(256) void slx_gstream_kernel(const SlxKParams p)
     const unsigned c = q % cpg, j = q / cpg;
     const unsigned Kq = p.sq_groups_total > j ? (p.sq_groups_total - j + m - 1u) / m : 0u;
     const unsigned Wq = (total_waves - q + NQ - 1u) / NQ;
-    const unsigned last_ticket = Kq + Wq - 1u;
-    unsigned *ctr = p.sq_counters + (size_t)q * 32u;
-    auto fetch_issue = [&](unsigned &raw) {
-        asm volatile("s_mov_b32 %0, 1\n\ts_atomic_add %0, %1, 0x0 glc" : "=&s"(raw) : "s"(ctr) : "memory");
-    };
-    auto fetch_wait = [&](unsigned &raw) { asm volatile("s_waitcnt lgkmcnt(0)" : "+s"(raw)::"memory"); };
-    auto reset_behind_last = [&](unsigned raw) {   // the queue's last ticket of the launch: the counter goes back to zero (slx_stream_kernel)
-        if (raw == last_ticket) asm volatile("s_atomic_and %0, %1, 0x0" ::"s"(0u), "s"(ctr) : "memory");
-    };
+    const TicketQueue queue(p.sq_counters, q, Kq, Wq);
 
     // ---- per-column state, once per launch
     const unsigned W = (unsigned)p.width, H = (unsigned)p.height;
@@ -1611,21 +1603,21 @@ __global__ __launch_bounds__(256) void slx_gstream_kernel(const SlxKParams p)
 
     // ---- items: ticket -> (frame-set, first row of the row group)
     struct Item { unsigned valid, set, row_base; };
-    auto decode = [&](unsigned raw) {
+    auto decode = [&](unsigned k) {
         Item it;
-        const unsigned k = raw;
         it.valid = k < Kq ? 1u : 0u;
         const unsigned G = it.valid ? k * m + j : 0u;
         it.set = p.sq_groups_per_set == 1u ? G : __umulhi(G, p.sq_magic);
         it.row_base = (G - it.set * p.sq_groups_per_set) * R * il;
         return it;
     };
-    unsigned raw;
-    fetch_issue(raw);
-    fetch_wait(raw);
-    reset_behind_last(raw);
-    Item A = decode(raw), B{0u, 0u, 0u};
-    if (!A.valid) return;
+    unsigned ticket = uniform_u32(queue.draw(lane));               // the newest ticket this wave has drawn
+    Item A = decode(ticket);
+    if (!A.valid) {
+        queue.reset_behind_last(ticket, lane);
+        return;
+    }
+    const unsigned second = queue.draw(lane);                      // arrives behind the first requests
 
     // request side (one row = two chunks ahead): its item, rows of it already requested, the two descriptors, lane offset of the next row
     Item D = A;
@@ -1638,46 +1630,29 @@ __global__ __launch_bounds__(256) void slx_gstream_kernel(const SlxKParams p)
         const unsigned voff = dma_off < dma_last ? dma_off : dma_last;
         uint32_t *dst = ring;
         unsigned so = p.phase_first;
-        if (p.dma_imm) {
-            static_for<NPH>([&](auto k) {
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(drsrc, (lds_void *)dst, 4, voff, so, decltype(k)::value * 256, 2 /* nt */);
-                if (decltype(k)::value + 1 < NPH) next_plane(so, p.phase_step - 256u);
-            });
-        } else {
-#pragma unroll
-            for (int k = 0; k < NPH; k++) {
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(drsrc, (lds_void *)(dst + k * 64), 4, voff, so, 0, 2 /* nt */);
-                if (k + 1 < NPH) next_plane(so, p.phase_step);
-            }
-        }
+        static_for<NPH>([&](auto k) {                              // (p.dma_imm: the plan takes this kernel only where it holds)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(drsrc, (lds_void *)dst, 4, voff, so, decltype(k)::value * 256, 2 /* nt */);
+            if (decltype(k)::value + 1 < NPH) next_plane(so, p.phase_step - 256u);
+        });
     };
     auto issue_gray = [&]() {                                      // ... its Gray planes into slot 1; the request side moves on a row
         const unsigned voff = dma_off < dma_last ? dma_off : dma_last;
         uint32_t *dst = ring + ROW_DW;
         unsigned so = 0u;
-        if (p.dma_imm) {
-            static_for<NGR>([&](auto k) {
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(dgrsrc, (lds_void *)dst, 4, voff, so, decltype(k)::value * 256, 2 /* nt */);
-                if (decltype(k)::value + 1 < NGR) next_plane(so, p.gray_step - 256u);
-            });
-        } else {
-#pragma unroll
-            for (int k = 0; k < NGR; k++) {
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(dgrsrc, (lds_void *)(dst + k * 64), 4, voff, so, 0, 2 /* nt */);
-                if (k + 1 < NGR) next_plane(so, p.gray_step);
-            }
-        }
+        static_for<NGR>([&](auto k) {
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(dgrsrc, (lds_void *)dst, 4, voff, so, decltype(k)::value * 256, 2 /* nt */);
+            if (decltype(k)::value + 1 < NGR) next_plane(so, p.gray_step - 256u);
+        });
         dma_off += dma_step;
         dri = uniform_u32(dri + 1u);
     };
     auto request_moves_to = [&](const Item &to) {
         D = to;
         dri = 0;
-        if (to.valid) {
-            drsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(uniform_ptr(p.plane_base + (size_t)to.set * p.phase_set_stride)), 0, 0xFFFFFFFFu, 0x00020000);
-            dgrsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(uniform_ptr(p.gray[0] + (size_t)to.set * p.gray_set_stride)), 0, 0xFFFFFFFFu, 0x00020000);
-            dma_off = dma_lane + to.row_base * row_stride;
-        }
+        const unsigned range = uniform_u32(to.valid ? 0xFFFFFFFFu : 0u);   // behind the last item: empty descriptors
+        drsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(uniform_ptr(p.plane_base + (size_t)to.set * p.phase_set_stride)), 0, range, 0x00020000);
+        dgrsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(uniform_ptr(p.gray[0] + (size_t)to.set * p.gray_set_stride)), 0, range, 0x00020000);
+        dma_off = dma_lane + to.row_base * row_stride;
     };
 
     // compute side: item A, row ri of it; where its rows are stored
@@ -1685,26 +1660,26 @@ __global__ __launch_bounds__(256) void slx_gstream_kernel(const SlxKParams p)
     unsigned row = A.row_base + sub;
     __amdgpu_buffer_rsrc_t zrsrc = __builtin_amdgcn_make_buffer_rsrc(p.z + (size_t)A.set * p.out_set_stride, 0, H * W * 8u, 0x00020000);
     unsigned out_boff[2] = {out_lane[0] + A.row_base * W * 8u, out_lane[1] + A.row_base * W * 8u};
-    __amdgpu_buffer_rsrc_t prsrc = zrsrc;
-    unsigned pend_off[2] = {0xFFFFFFF0u, 0xFFFFFFF0u};
+    // no row staged yet: an empty descriptor drops the first step's stores
+    __amdgpu_buffer_rsrc_t prsrc = __builtin_amdgcn_make_buffer_rsrc(p.z, 0, 0u, 0x00020000);
+    unsigned pend_off[2] = {0u, 0u};
+    auto flush_row = [&]() {
+#pragma unroll
+        for (int k = 0; k < NZ; k++) {
+            const u32x4 v = *reinterpret_cast<const u32x4 *>(stage + k * 64 + lane);
+            __builtin_amdgcn_raw_buffer_store_b128(v, prsrc, pend_off[k], 0, 2 /* nt */);
+        }
+    };
     issue_phase();                                                 // row 0 of the first item
     issue_gray();
-    for (unsigned s = 0;; s++) {
+    ticket = uniform_u32(second);
+    Item B = decode(ticket);
+    for (;;) {
         __builtin_amdgcn_s_setprio(1);                             // (slx_stream_kernel: priority up to the step's last DMA request)
-        unsigned next_raw;                                         // the ticket of the item after this one: a variable of this step alone (see slx_stream_kernel)
-        if (ri == 0) fetch_issue(next_raw);
-        // ---- chunk 0: the row's phase planes.  Behind their DMA only the row's Gray DMA has been issued
+        // ---- chunk 0: the row's phase planes.  Behind their DMA: the ticket drawn last step (retired with it) and the row's Gray DMA
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NGR) : "memory");
-        if (s > 0) {                                               // last row's stores, one step late
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const u32x4 v = *reinterpret_cast<const u32x4 *>(stage + k * 64 + lane);
-                __builtin_amdgcn_raw_buffer_store_b128(v, prsrc, pend_off[k], 0, 2 /* nt */);
-            }
-        }
-        // No divergent branch between the ticket's issue and its wait: rows past the tile run the phase arithmetic on the last row's
-        // bytes (their DMA is clamped to it) and are never stored.  (With `if (row < H)` around it hipcc carried the in-flight ticket
-        // through a VECTOR register across the branch -- a copy of the placeholder, which the compiler then could not even lower.)
+        flush_row();                                               // last row's stores, one step late
+        // rows past the tile run the phase arithmetic on the last row's bytes (their DMA is clamped to it) and are never stored
         float pix[SLX_QUAD];
         {
             const uint32_t *src = ring + lane;
@@ -1718,21 +1693,15 @@ __global__ __launch_bounds__(256) void slx_gstream_kernel(const SlxKParams p)
             pix[2] = px.b.x;
             pix[3] = px.b.y;
         }
-        // slot 0 is free once it has been read -- and the ticket requested above has arrived with the same wait
-        if (ri == 0) {
-            fetch_wait(next_raw);
-            reset_behind_last(next_raw);
-            B = decode(next_raw);
-        } else {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");         // slot 0 is free once it has been read
         if (D.valid && dri == R) request_moves_to(B);
-        const unsigned more = uniform_u32(D.valid);                // is there a row after this one?
-        if (more) issue_phase();
+        issue_phase();
         // ---- chunk 1: the row's Gray planes.  Behind their DMA: the stores above and the phase DMA just issued
-        if (!more) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        else if (s > 0) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NPH + NZ) : "memory");
-        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NPH) : "memory");
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NPH + NZ) : "memory");
+        // the ticket of the item after B, drawn at A's last row and used at the end of this step
+        const bool last_row = ri + 1u == R;
+        unsigned next = ~0u;
+        if (last_row && B.valid) next = queue.draw(lane);
         uint32_t gw[NGR];
         {
             const uint32_t *src = ring + ROW_DW + lane;
@@ -1740,7 +1709,7 @@ __global__ __launch_bounds__(256) void slx_gstream_kernel(const SlxKParams p)
             for (int k = 0; k < NGR; k++) gw[k] = src[k * 64];
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");         // slot 1 is free once it has been read
-        if (more) issue_gray();
+        issue_gray();
         __builtin_amdgcn_s_setprio(0);
         if (row < H) {
             // a3 + the bit-pack of a4 on the whole quad (slx_strip_kernel)
@@ -1779,9 +1748,11 @@ __global__ __launch_bounds__(256) void slx_gstream_kernel(const SlxKParams p)
         __builtin_amdgcn_wave_barrier();
         // next row of the item, or the next item
         ri = uniform_u32(ri + 1u);
-        if (ri == R) {
+        if (last_row) {
             if (!B.valid) break;
             A = B;
+            ticket = uniform_u32(next);
+            B = decode(ticket);
             ri = 0;
             row = A.row_base + sub;
             zrsrc = __builtin_amdgcn_make_buffer_rsrc(uniform_ptr(p.z + (size_t)A.set * p.out_set_stride), 0, H * W * 8u, 0x00020000);
@@ -1793,12 +1764,10 @@ __global__ __launch_bounds__(256) void slx_gstream_kernel(const SlxKParams p)
             out_boff[1] += out_step;
         }
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-        const u32x4 v = *reinterpret_cast<const u32x4 *>(stage + k * 64 + lane);
-        __builtin_amdgcn_raw_buffer_store_b128(v, prsrc, pend_off[k], 0, 2 /* nt */);
-    }
+    // no DMA may land in LDS behind the wave's end, the empty ones of the last steps included
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    flush_row();
+    queue.reset_behind_last(ticket, lane);
 }
 
 // ------------------------------------------------------------------------------------------

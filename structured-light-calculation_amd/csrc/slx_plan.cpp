@@ -248,9 +248,9 @@ int slx_plan_launch(const SlxKParams &kp_in, int mode, bool aux, int n_sets, int
     }
     // Stream kernel (slx_kernels.hip: slx_stream_kernel): the Gray-free 4-step depth-only class, launches that fill the chip many times over.
     // (An instantiation with the optional planes x, y, U, k was built and measured in round 5 -- C4 x 8 / 16 / 32 frame-sets: +1.5 / -1.6 /
-    // -0.6 % against the strip kernel on the same box -- and is not in the tree: profiles/experiments/r05_stream_kernel_optional_planes.patch.)
+    // -0.6 % against the strip kernel on the same box -- and is not in the tree.)
     plan->stream = 0;
-    if (!decoder && mode == SLX_MODE_MULTIFREQ && kp.n_steps == 4 && !aux && kp.sq_counters && tn.stream != 1 && tn.weave <= 1) {
+    if (!decoder && mode == SLX_MODE_MULTIFREQ && kp.n_steps == 4 && kp.dma_imm && !aux && kp.sq_counters && tn.stream != 1 && tn.weave <= 1) {
         const unsigned il = 64u / g;                                     // no weave: the queues hand the rows out in order anyway
         const unsigned cpg = il * QR / 64u;
         const unsigned R = (tn.stream_rows >= 2 && tn.stream_rows <= 16) ? (unsigned)tn.stream_rows : 2u;   // measured: 2 rows 270, 4: 274, 8: 284, 16: 302 us (C4 x 32)
@@ -299,7 +299,7 @@ int slx_plan_launch(const SlxKParams &kp_in, int mode, bool aux, int n_sets, int
     // Same queues and counters as slx_stream_kernel; a row is two ring chunks there, an item ONE row (REF x 32: 164.3 us with 1-row
     // items, 171.3 with 2, 177.6 with 3: profiles/r06_gstream_ab.log).  Taken from 8 items per resident wave on -- same-box against the
     // strip kernel: 32 frame-sets of the reference's size -3.1 %, 16 -3.5 %, 8 -2.4 %, 4 (5 items per wave) +0.7 %.
-    if (!decoder && gb == 6 && mode == SLX_MODE_GRAY_PHASE && kp.n_steps == 4 && !aux && kp.sq_counters && tn.stream != 1 && tn.weave <= 1) {
+    if (!decoder && gb == 6 && mode == SLX_MODE_GRAY_PHASE && kp.n_steps == 4 && kp.dma_imm && !aux && kp.sq_counters && tn.stream != 1 && tn.weave <= 1) {
         const unsigned il = 64u / g, cpg = il * QR / 64u;
         const unsigned R = (tn.stream_rows >= 1 && tn.stream_rows <= 16) ? (unsigned)tn.stream_rows : 1u;
         const unsigned gps = ((unsigned)kp.height + R * il - 1u) / (R * il);

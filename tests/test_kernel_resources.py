@@ -107,130 +107,134 @@ def test_planner_occupancy_matches_compiled_register_counts(kernels):
         assert claimed == min(8 if mode in (0, 1) else 4, allowed), ((mode, F, GB, NS, AUX), v["vgpr_count"], claimed, allowed)
 
 
-def _sgprs(operand_text):
-    """Indices of every scalar register an operand list names (s5, s[4:7])."""
+def _blocks_of(lines, mangled):
+    """Basic blocks (lists of instructions) of one compiled kernel and each block's successors.  A wait written in the source (inline
+    assembly) is marked `asm:`, hipcc's own are not."""
+    start = next(i for i, ln in enumerate(lines) if re.match(r"^_ZN\S*%s:" % mangled, ln))
+    end = next(i for i in range(start, len(lines)) if lines[i].startswith(".Lfunc_end"))
+    blocks, label_of, in_asm = [[]], {}, False
+    for raw in lines[start + 1:end]:
+        in_asm = "#ASMSTART" in raw or (in_asm and "#ASMEND" not in raw)
+        ln = raw.split(";")[0].rstrip()
+        m = re.match(r"^(\.LBB\S*):", ln)
+        if m:
+            if blocks[-1]:
+                blocks.append([])
+            label_of[m.group(1)] = len(blocks) - 1
+            continue
+        if not ln.startswith("\t") or ln.strip().startswith("."):
+            continue
+        t = ln.strip()
+        blocks[-1].append("asm:" + t if in_asm and t.startswith("s_waitcnt") else t)
+        if t.startswith(("s_cbranch", "s_branch", "s_endpgm")):
+            blocks.append([])
+    succ = []
+    for b, insts in enumerate(blocks):
+        last = insts[-1] if insts else ""
+        nxt = [b + 1] if b + 1 < len(blocks) else []
+        if last.startswith("s_endpgm"):
+            succ.append([])
+        elif last.startswith("s_branch"):
+            succ.append([label_of[last.split()[1]]])
+        elif last.startswith("s_cbranch"):
+            succ.append(nxt + [label_of[last.split()[1]]])
+        else:
+            assert not last.startswith(("s_setpc", "s_swappc")), (mangled, last)
+            succ.append(nxt)
+    return blocks, succ
+
+
+def _vgprs(operand_text):
+    """Indices of every vector register an operand list names (v5, v[4:7])."""
     regs = set()
-    for m in re.finditer(r"\bs\[(\d+):(\d+)\]", operand_text):
+    for m in re.finditer(r"\bv\[(\d+):(\d+)\]", operand_text):
         regs.update(range(int(m.group(1)), int(m.group(2)) + 1))
-    for m in re.finditer(r"\bs(\d+)\b", operand_text):
+    for m in re.finditer(r"\bv(\d+)\b", operand_text):
         regs.add(int(m.group(1)))
     return regs
 
 
+def _vmem_tag(t):
+    """What an instruction adds to the vmcnt sequence: 'T<reg>' a ticket, 'L<descriptor>' a DMA into LDS, 'Z' a buffer store, 'S' a global
+    store, 'G' any other load; None for everything else."""
+    op, _, rest = t.partition(" ")
+    assert not op.startswith(("flat_", "scratch_", "tbuffer_")), t
+    if op.startswith(("global_atomic", "buffer_atomic")):
+        assert op == "global_atomic_add" and " sc0" in t, t               # the ticket is the only atomic, and it returns the old value
+        return "T%d" % min(_vgprs(rest.split(",")[0]))
+    if op.startswith("buffer_load"):
+        return "L" + re.search(r"s\[\d+:\d+\]", rest).group(0) if t.endswith(" lds") else "G"
+    if op.startswith("buffer_store"):
+        return "Z"
+    if op.startswith("global_store"):
+        return "S"
+    return "G" if op.startswith("global_load") else None
+
+
 def test_stream_kernel_ticket_register_is_untouched_between_issue_and_wait(tmp_path):
-    """slx_stream_kernel takes its work tickets with a scalar atomic whose result lands in an SGPR when the NEXT `s_waitcnt lgkmcnt(0)`
-    retires -- issue and wait are two asm statements with the step's DMA wait, the depth stores and the LDS reads between them
-    (csrc/slx_kernels.hip: fetch_issue / fetch_wait).  The register allocator knows the variable is live across that window, so it
-    gives the register to nothing else there; what it does NOT know is that the value is still in flight: a copy or a spill of it
-    inside the window (a phi of the `if (ri == 0)` arms, scalar-register pressure) would read the placeholder (1) instead of the
-    ticket, and rows would be skipped or decoded twice with no error.  This pins the compiled code of every instantiation:
-      * every s_atomic_add writes a register R directly behind `s_mov_b32 R, 1` (two ticket variables: the entry ticket, the loop's);
-      * no instruction READS R at a point an in-flight ticket can reach: "in flight" is set by the issue, cleared by an
-        `s_waitcnt ... lgkmcnt(0)` or another definition of R, and propagated over the control-flow graph to a fixed point (the
-        optional-plane instantiations are short of scalar registers and reuse R for other values outside the window: those uses
-        are clear of it by construction of the walk)."""
+    """The stream kernels take their work tickets with a vector atomic whose result comes back in the vmcnt sequence that their DMA ring
+    counts (csrc/slx_kernels.hip: TicketQueue).  This walks the compiled code of every instantiation with the exact sequence of
+    outstanding vector-memory operations as the state (every path through the control-flow graph, arms that exclude each other
+    included: that can only add states):
+      * no instruction reads or writes a ticket's register while its atomic is outstanding;
+      * what each counted wait of the ring leaves in flight is exactly what the source says: one row's stores and the next chunk
+        (slx_stream_kernel); the row's Gray chunk, or one row's stores and the next phase chunk (slx_gstream_kernel) -- so the chunk
+        that is read next has landed whole;
+      * the wait hipcc puts in front of the ticket's use takes nothing else out of flight in slx_stream_kernel's loop;
+      * no DMA into LDS is outstanding when a wave ends."""
     if not os.path.exists(HIPCC):
         pytest.skip("hipcc is not installed")
     out = str(tmp_path / "slx_kernels.s")
     subprocess.check_call([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-I" + os.path.join(ROOT, "include"),
                            "-I" + CSRC, "-S", "--cuda-device-only", os.path.join(CSRC, "slx_kernels.hip"), "-o", out], stderr=subprocess.DEVNULL)
     lines = open(out).read().split("\n")
-    ticket_reads = 0
-    instantiations = [("slx_stream_kernelILi%dEEEv10SlxKParams" % F, "slx_stream_kernel<%d>" % F) for F in (1, 2, 3, 4)]
-    instantiations += [("slx_gstream_kernelE10SlxKParams", "slx_gstream_kernel")]
-    for mangled, who in instantiations:
-        start = next(i for i, ln in enumerate(lines) if re.match(r"^_ZN\S*%s:" % mangled, ln))
-        end = next(i for i in range(start, len(lines)) if lines[i].startswith(".Lfunc_end"))
-        body = [ln.split(";")[0].rstrip() for ln in lines[start + 1:end]]
-        # basic blocks: a label starts one, a branch / s_endpgm ends one
-        blocks, label_of = [[]], {}
-        for ln in body:
-            m = re.match(r"^(\.LBB\S*):", ln)
-            if m:
-                if blocks[-1]:
-                    blocks.append([])
-                label_of[m.group(1)] = len(blocks) - 1
+    NZ = 2
+    kernels = [("slx_stream_kernelILi%dEEEv10SlxKParams" % F, "slx_stream_kernel<%d>" % F, 4 * F, 0) for F in (1, 2, 3, 4)]
+    kernels += [("slx_gstream_kernelE10SlxKParams", "slx_gstream_kernel", 4, 12)]
+    for mangled, who, nph, ngr in kernels:
+        blocks, succ = _blocks_of(lines, mangled)
+        draws = [t for insts in blocks for t in insts if t.startswith("global_atomic_add ")]
+        assert len(draws) >= 3, (who, "expected the first two tickets and the loop's")
+        ring_waits = {}
+        seen = [set() for _ in blocks]
+        work = [(0, ())]
+        while work:
+            b, queue = work.pop()
+            if queue in seen[b]:
                 continue
-            if not ln.startswith("\t") or ln.strip().startswith("."):
-                continue
-            t = ln.strip()
-            blocks[-1].append(t)
-            if t.startswith(("s_cbranch", "s_branch", "s_endpgm")):
-                blocks.append([])
-        succ = []
-        for b, insts in enumerate(blocks):
-            last = insts[-1] if insts else ""
-            nxt = [b + 1] if b + 1 < len(blocks) else []
-            if last.startswith("s_endpgm"):
-                succ.append([])
-            elif last.startswith("s_branch"):
-                succ.append([label_of[last.split()[1]]])
-            elif last.startswith("s_cbranch"):
-                succ.append(nxt + [label_of[last.split()[1]]])
-            else:
-                assert not last.startswith(("s_setpc", "s_swappc")), (who, last)
-                succ.append(nxt)
-        atomics = [t for insts in blocks for t in insts if t.startswith("s_atomic_add ")]
-        assert len(atomics) >= 2, (who, "expected the entry ticket and the loop's ticket")
-        dest = sorted({int(re.match(r"s_atomic_add s(\d+),", t).group(1)) for t in atomics})
-        assert len(dest) <= 2, (who, "more ticket registers than ticket variables (the entry ticket, the loop's): a copy of a pending register", dest)
-        for R in dest:
-            mov = "s_mov_b32 s%d, 1" % R
-
-            def operands(t):
-                op, _, rest = t.partition(" ")
-                return op, [o.strip() for o in rest.split(",")] if rest else []
-
-            def writes_R(t):
-                op, ops = operands(t)
-                if not ops or op.startswith(("s_cmp", "s_bitcmp", "s_waitcnt", "s_cbranch", "s_branch", "buffer_store", "global_store", "ds_write", "s_setprio", "s_nop")):
-                    return False
-                return R in _sgprs(ops[0])                               # ALU / scalar loads / the atomic: operand 0 is the destination
-
-            def reads_R(t):
-                op, ops = operands(t)
-                if t.startswith("s_atomic_add s%d," % R):
-                    return False                                          # its data operand is the placeholder the s_mov just wrote: the issue itself
-                srcs = ops if op.startswith(("s_cmp", "s_bitcmp", "buffer_store", "global_store", "ds_write")) else ops[1:]
-                return any(R in _sgprs(o) for o in srcs)
-            # "a ticket may be in flight in R": set by the issue, cleared by an lgkmcnt(0) wait (the ticket has landed: R then holds an
-            # ordinary value) or by another definition of R; propagated along fall-through and branch edges to a fixed point.  The walk
-            # is path-insensitive (it also follows arm combinations the `ri == 0` tests exclude), which can only add windows, never hide one.
-            def step(t, state):
-                if t.startswith("s_atomic_add s%d," % R) or t == mov:
-                    return True
-                if (t.startswith("s_waitcnt") and "lgkmcnt(0)" in t) or writes_R(t):
-                    return False
-                return state
-            pend_in = [False] * len(blocks)
-            changed = True
-            while changed:
-                changed = False
-                for b, insts in enumerate(blocks):
-                    state = pend_in[b]
-                    for t in insts:
-                        state = step(t, state)
-                    for nb in succ[b]:
-                        if state and not pend_in[nb]:
-                            pend_in[nb] = True
-                            changed = True
-            for b, insts in enumerate(blocks):
-                state = pend_in[b]
-                for k, t in enumerate(insts):
-                    if t.startswith("s_atomic_add s%d," % R):
-                        assert k > 0 and insts[k - 1] == mov, (who, "the placeholder is not written directly before the atomic", insts[max(0, k - 2):k + 1])
-                    if reads_R(t):
-                        assert not state, (who, "s%d is read where a ticket may still be in flight" % R, t, insts[max(0, k - 6):k + 1])
-                        consumed = False                             # the consuming read: directly behind the wait, in its block
-                        for tj in reversed(insts[:k]):
-                            if tj.startswith("s_waitcnt") and "lgkmcnt(0)" in tj:
-                                consumed = True
-                                break
-                            if writes_R(tj) or tj.startswith("s_atomic_add"):
-                                break
-                        ticket_reads += 1 if consumed else 0
-                    state = step(t, state)
-    assert ticket_reads >= 10                                         # the entry ticket's and the loop ticket's consumption, all 5 kernels
+            seen[b].add(queue)
+            assert sum(map(len, seen)) < 200000, (who, "the walk does not converge")
+            for k, t in enumerate(blocks[b]):
+                if t.startswith(("s_waitcnt", "asm:s_waitcnt")):
+                    m = re.search(r"vmcnt\((\d+)\)", t)
+                    if not m:
+                        continue
+                    n = int(m.group(1))
+                    queue = queue[max(0, len(queue) - n):]
+                    if t.startswith("asm:") and n:
+                        dma = queue[-1:]                                   # its descriptor: all of a chunk's
+                        want = {nph + NZ: ("Z",) * NZ + dma * nph, ngr: dma * ngr}[n]   # one row's stores and the next (phase) chunk; the Gray chunk
+                        assert queue == want[max(0, len(want) - len(queue)):], (who, t, queue)
+                        ring_waits[b, k] = max(ring_waits.get((b, k), 0), len(queue))
+                    continue
+                touched = _vgprs(t.partition(" ")[2])
+                for q in queue:
+                    assert q[0] != "T" or int(q[1:]) not in touched, (who, "v%s is touched while its ticket is in flight" % q[1:], t, queue)
+                tag = _vmem_tag(t)
+                if tag:
+                    queue = (queue + (tag,))[-63:]
+                if t.startswith("s_endpgm"):
+                    assert not any(q[0] == "L" for q in queue), (who, "a DMA may land behind the wave's end", queue)
+            for nb in succ[b]:
+                work.append((nb, queue))
+        # the loop's one counted wait (slx_stream_kernel), its two (slx_gstream_kernel): each was reached with all of that in flight
+        assert sorted(ring_waits.values()) == sorted({nph + NZ, ngr} - {0}), (who, ring_waits)
+        reads = {m.group(1) for insts in blocks for t in insts for m in [re.match(r"v_readfirstlane_b32 s\d+, v(\d+)", t)] if m}
+        assert {re.match(r"global_atomic_add v(\d+),", t).group(1) for t in draws} <= reads, (who, "every ticket is read through one lane")
+        if ngr == 0:
+            loop = min(ring_waits)[0]                                     # the block with the loop's counted wait, and everything behind it
+            own = [int(m.group(1)) for insts in blocks[loop:] for t in insts for m in [re.match(r"s_waitcnt.*vmcnt\((\d+)\)", t)] if m]
+            assert own and min(own) >= nph + NZ, (who, "a wait of hipcc's in the loop drains the ring", own)
 
 
 def test_fused_cloud_kernel_registers_match_the_plan(tmp_path):

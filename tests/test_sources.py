@@ -1,6 +1,7 @@
 """What the tree's text may not hold, checked on the files themselves (CPU only).
 
-Statements about the reference rest on its sources, build files and documents, never on what its prebuilt executables contain.
+Statements about the reference rest on its sources, build files and documents, never on what its prebuilt executables contain; GPU code
+writes through the vector path only.
 """
 import os
 import re
@@ -29,5 +30,11 @@ def _hits(pattern, *suffixes):
 
 def test_no_document_cites_the_contents_of_a_prebuilt_executable():
     """A tool's output on a shipped .exe / .dll, or its import table, is no source of a statement here."""
-    reads = r"(?i)(`strings`|import (table|visible)|imports? of|dumpbin|objdump|readelf).{0,120}\.(exe|dll)\b|\.(exe|dll)\b.{0,60}(import table|confirmed by|disassembl)"
+    reads = r"(?i)confirmed by `(strings|objdump|readelf|dumpbin)` on|(import|imports|symbol) visible in `[^`]*\.(exe|dll)"
     assert _hits(reads, ".md") == []
+
+
+def test_no_gpu_code_writes_through_the_scalar_cache():
+    """Scalar stores and atomics, the scalar cache's write-back and discard: in no source, script, test or kept patch, not as a comment."""
+    writes = r"\b(?:s_(?:buffer_|scratch_)?(?:atomic|store)(?=_)|s_d" + r"cache_(?:wb|discard))"
+    assert _hits(writes, ".hip", ".cpp", ".hpp", ".h", ".c", ".s", ".py", ".sh", ".patch", "Makefile", ".mk", ".txt") == []
