@@ -45,28 +45,15 @@ constexpr float kInv360 = 1.0f / 360.0f;
 __device__ __forceinline__ float ubyte(uint32_t w, int j) { return (float)((w >> (8 * j)) & 0xffu); }
 __device__ __forceinline__ int ibyte(uint32_t w, int j) { return (int)((w >> (8 * j)) & 0xffu); }
 
-// Two pixels at a time with explicit 2-vectors, so that every multiply / add / fma of the sequence is a packed
-// instruction (v_pk_*_f32 retire two lanes' worth per issue slot); compares and selects stay per component.
+// Two pixels at a time with explicit 2-vectors.  No operation on them is a packed f32 instruction: those have given wrong results on this
+// hardware, the build turns them off for hipcc (-packed-fp32-ops in the Makefile), and the assembly below writes one pixel at a time.
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-// saturate(-a) and saturate(a * s) to [0, 1], both halves in one packed instruction
-__device__ __forceinline__ f32x2 pk_neg_sat(f32x2 a)
-{
-    f32x2 r;
-    asm("v_pk_mul_f32 %0, %1, -1.0 op_sel_hi:[1,0] clamp" : "=v"(r) : "v"(a));
-    return r;
-}
-__device__ __forceinline__ f32x2 pk_mul_sat(f32x2 a, f32x2 s)
-{
-    f32x2 r;
-    asm("v_pk_mul_f32 %0, %1, %2 clamp" : "=v"(r) : "v"(a), "v"(s));
-    return r;
-}
 // (byte J of a) - (byte J of b) in one VALU slot (SDWA operand selects); hipcc finds this form
 // for only some of the 24 differences of a row step.
 // Byte J of a minus byte J of b as a float, times 2^-149: the SDWA byte select zero-extends the byte into the float
 // operand, where it is the denormal byte * 2^-149, and the subtraction of two denormals is exact (f32 denormals are on:
 // .amdhsa_float_denorm_mode_32 3, hipcc's default for gfx9).  One instruction instead of an integer SDWA subtraction
-// plus v_cvt_f32_i32; the caller rescales two such differences with one packed multiply.
+// plus v_cvt_f32_i32; the caller rescales it with one multiply.
 template <int J>
 __device__ __forceinline__ float byte_diff_denorm(uint32_t a, uint32_t b)
 {
@@ -109,10 +96,8 @@ __device__ __forceinline__ int byte_diff(uint32_t a, uint32_t b)
 //  * (float)((double)q * (double)T) == q*T in f32 (the double product is exact), and
 //    (float)((double)pix + 0.5) == pix + 0.5f (the double sum is exact for pix = 0 or >= 2^-11).
 // ---- the phase arithmetic on vectors of pixels ---------------------------------------------------------------------
-// f32x2 operands make every multiply / add / fma a packed instruction (two pixels per issue slot).  F32x2x2 is two such
-// pairs evaluated in LOCKSTEP: every operation is issued for pair a, then for pair b.  Dependent packed operations need a
-// wait state between them -- hipcc pads with s_nop, and an s_nop costs the wave an issue turn like a real instruction
-// (122 per row before, 14 after) -- and the other pair's independent operation fills it.
+// F32x2x2 is a quad as two pixel pairs evaluated in LOCKSTEP: every operation is issued for pair a, then for pair b, so that four
+// independent chains interleave and none waits for its own last result.
 struct F32x2x2 {
     f32x2 a, b;
 };
@@ -134,12 +119,10 @@ __device__ __forceinline__ f32x2 v_max(f32x2 x, f32x2 y) { return {__builtin_fma
 __device__ __forceinline__ f32x2 v_max3(f32x2 x, f32x2 y, float z) { return {__builtin_fmaxf(__builtin_fmaxf(x.x, y.x), z), __builtin_fmaxf(__builtin_fmaxf(x.y, y.y), z)}; }
 __device__ __forceinline__ f32x2 v_min(f32x2 x, f32x2 y) { return {__builtin_fminf(x.x, y.x), __builtin_fminf(x.y, y.y)}; }
 __device__ __forceinline__ f32x2 v_rcp(f32x2 x) { return {__builtin_amdgcn_rcpf(x.x), __builtin_amdgcn_rcpf(x.y)}; }
-__device__ __forceinline__ f32x2 v_mul_sat(f32x2 x, float s) { return pk_mul_sat(x, f32x2{s, s}); }
-__device__ __forceinline__ f32x2 v_neg_sat(f32x2 x) { return pk_neg_sat(x); }
 
 // ---- selects as arithmetic on 2-cycle instructions --------------------------------------------------------------
 // tools/valubench.hip: a wave's plain v_mul_f32 / v_add_f32 (also with |x| or clamp modifiers) issue in 2 cycles, v_fma_f32
-// in ~3.5, every packed f32 operation, v_cmp, v_cndmask, v_min / v_max in 4.  A compare + select of a pixel pair costs 16
+// in ~3.5, v_cmp, v_cndmask, v_min / v_max in 4.  A compare + select of a pixel pair costs 16
 // cycles; the forms below cost 8 or less.
 // sat(x * s), one pixel: v_mul_f32 ... clamp (hipcc has no source form for the clamp bit)
 __device__ __forceinline__ float mul_sat1(float x, float s)
@@ -148,13 +131,27 @@ __device__ __forceinline__ float mul_sat1(float x, float s)
     asm("v_mul_f32_e64 %0, %1, %2 clamp" : "=v"(r) : "v"(x), "s"(s));
     return r;
 }
+__device__ __forceinline__ float neg_sat1(float x)
+{
+    float r;
+    asm("v_mul_f32_e64 %0, %1, -1.0 clamp" : "=v"(r) : "v"(x));
+    return r;
+}
+// sat(-x * s), one pixel: the sign rides as a source modifier, so that s is the scalar register the other saturations use
+__device__ __forceinline__ float negmul_sat1(float x, float s)
+{
+    float r;
+    asm("v_mul_f32_e64 %0, -%1, %2 clamp" : "=v"(r) : "v"(x), "s"(s));
+    return r;
+}
+__device__ __forceinline__ f32x2 v_negmul_sat(f32x2 x, float s) { return {negmul_sat1(x.x, s), negmul_sat1(x.y, s)}; }
+__device__ __forceinline__ f32x2 v_neg_sat(f32x2 x) { return {neg_sat1(x.x), neg_sat1(x.y)}; }
 // 1.0 where |p| > |q|, else 0.0 (both 0 or separated by far more than 2^-60: every caller's operands are)
 __device__ __forceinline__ f32x2 v_gt01_abs(f32x2 p, f32x2 q)
 {
     return {mul_sat1(__builtin_fabsf(p.x) - __builtin_fabsf(q.x), 0x1p60f), mul_sat1(__builtin_fabsf(p.y) - __builtin_fabsf(q.y), 0x1p60f)};
 }
-// fma(k, m, |z|) per pixel: v_fma_f32 with the |.| modifier on the addend (VOP3P has no abs; written as asm because hipcc's
-// vectoriser otherwise pairs the two fmas into a v_pk_fma_f32 behind two v_and_b32)
+// fma(k, m, |z|) per pixel: v_fma_f32 with the |.| modifier on the addend
 __device__ __forceinline__ float fma_absz1(float k, float m, float z)
 {
     float r;
@@ -170,14 +167,14 @@ __device__ __forceinline__ float absmul1(float x, float s)
     return r;
 }
 __device__ __forceinline__ f32x2 v_absmul(f32x2 x, float s) { return {absmul1(x.x, s), absmul1(x.y, s)}; }
-// sat(fma(x, y, z)), both halves in one packed instruction
-__device__ __forceinline__ f32x2 pk_fma_sat(f32x2 x, f32x2 y, f32x2 z)
+// sat(fma(x, y, z)) per pixel: v_fma_f32 ... clamp (one scalar register operand per instruction: z in a vector one)
+__device__ __forceinline__ float fma_sat1(float x, float y, float z)
 {
-    f32x2 r;
-    asm("v_pk_fma_f32 %0, %1, %2, %3 clamp" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+    float r;
+    asm("v_fma_f32 %0, %1, %2, %3 clamp" : "=v"(r) : "v"(x), "s"(y), "v"(z));
     return r;
 }
-__device__ __forceinline__ f32x2 v_fma_sat(f32x2 x, float y, float z) { return pk_fma_sat(x, f32x2{y, y}, f32x2{z, z}); }
+__device__ __forceinline__ f32x2 v_fma_sat(f32x2 x, float y, float z) { return {fma_sat1(x.x, y, z), fma_sat1(x.y, y, z)}; }
 
 #define SLX_LOCKSTEP1(NAME) __device__ __forceinline__ F32x2x2 NAME(F32x2x2 x) { return {NAME(x.a), NAME(x.b)}; }
 SLX_LOCKSTEP1(v_abs)
@@ -192,7 +189,7 @@ __device__ __forceinline__ F32x2x2 v_fma(F32x2x2 x, F32x2x2 y, float z) { return
 __device__ __forceinline__ F32x2x2 v_max(F32x2x2 x, F32x2x2 y) { return {v_max(x.a, y.a), v_max(x.b, y.b)}; }
 __device__ __forceinline__ F32x2x2 v_max3(F32x2x2 x, F32x2x2 y, float z) { return {v_max3(x.a, y.a, z), v_max3(x.b, y.b, z)}; }
 __device__ __forceinline__ F32x2x2 v_min(F32x2x2 x, F32x2x2 y) { return {v_min(x.a, y.a), v_min(x.b, y.b)}; }
-__device__ __forceinline__ F32x2x2 v_mul_sat(F32x2x2 x, float s) { return {v_mul_sat(x.a, s), v_mul_sat(x.b, s)}; }
+__device__ __forceinline__ F32x2x2 v_negmul_sat(F32x2x2 x, float s) { return {v_negmul_sat(x.a, s), v_negmul_sat(x.b, s)}; }
 __device__ __forceinline__ F32x2x2 v_gt01_abs(F32x2x2 p, F32x2x2 q) { return {v_gt01_abs(p.a, q.a), v_gt01_abs(p.b, q.b)}; }
 __device__ __forceinline__ F32x2x2 v_fma_absz(float k, F32x2x2 m, F32x2x2 z) { return {v_fma_absz(k, m.a, z.a), v_fma_absz(k, m.b, z.b)}; }
 __device__ __forceinline__ F32x2x2 v_absmul(F32x2x2 x, float s) { return {v_absmul(x.a, s), v_absmul(x.b, s)}; }
@@ -241,8 +238,8 @@ __device__ __forceinline__ V wrapped_pix_from_diffs(V s2, V c2, float Tf)
     const V c = v_fma(v_fma(-mx, q0, mn), r, q0);                   // RN(mn / mx)
     const V cc = c * c;
     const V a = (((kP7 * cc + kP5) * cc + kP3) * cc + kP1) * c;
-    const V mc = SCALED ? v_mul_sat(c2, -0x1p60f) : v_neg_sat(c2);
-    const V ms = SCALED ? v_mul_sat(s2, -0x1p60f) : v_neg_sat(s2);
+    const V mc = SCALED ? v_negmul_sat(c2, 0x1p60f) : v_neg_sat(c2);
+    const V ms = SCALED ? v_negmul_sat(s2, 0x1p60f) : v_neg_sat(s2);
     return pix_from_octant_angle(a, v_gt01_abs(s2, c2), mc, ms, Tf);
 }
 
@@ -646,7 +643,7 @@ __device__ __forceinline__ V pix_tail_inrange(V y, V x, float Tf)
     const V c = v_fma(v_fma(-dd, q, mn), r, q);
     const V cc = c * c;
     const V a = (((kP7 * cc + kP5) * cc + kP3) * cc + kP1) * c;
-    return pix_from_octant_angle(a, v_gt01_abs(y, x), v_mul_sat(x, -0x1p60f), v_mul_sat(y, -0x1p60f), Tf);
+    return pix_from_octant_angle(a, v_gt01_abs(y, x), v_negmul_sat(x, 0x1p60f), v_negmul_sat(y, 0x1p60f), Tf);
 }
 
 // a3 for the four pixels of a quad at once (R/CDecodeGray.cpp:150-176: bit = pattern > inverse, ties -> 0), on the dwords
@@ -1051,7 +1048,7 @@ __global__ __launch_bounds__(256) void slx_strip_kernel(const SlxKParams p)
                 for (int f = 0; f < ((NS == 4 && c == 0) ? F : 0); f++) {
                     const uint32_t w0 = src[(f * 4 + 0) * 64], w1 = src[(f * 4 + 1) * 64];
                     const uint32_t w2 = src[(f * 4 + 2) * 64], w3 = src[(f * 4 + 3) * 64];
-                    // differences as denormals (x 2^-149), rescaled to x 2^-23 by one packed multiply per pair
+                    // differences as denormals (x 2^-149), rescaled to x 2^-23
                     const f32x2 kUp = {0x1p126f, 0x1p126f};
                     const F32x2x2 px = wrapped_pix_from_diffs<true>(
                         F32x2x2{f32x2{byte_diff_denorm<0>(w0, w2), byte_diff_denorm<1>(w0, w2)} * kUp, f32x2{byte_diff_denorm<2>(w0, w2), byte_diff_denorm<3>(w0, w2)} * kUp},
@@ -1306,7 +1303,7 @@ struct TicketQueue {
 //     no item left, they go to an empty descriptor (num_records 0: nothing is read or stored).  The counted waits are
 //     then one constant, and hipcc's own wait in front of the ticket's use counts to the same operations instead of draining the ring
 //     (tests/test_kernel_resources.py walks the compiled code).
-// Same box, against the strip kernel: C4 x 32 283.4 -> 271.7 us (5.43 TB/s of planes in and depth out), x 8 80.3 -> 74.1, C2 x 80 287.9 -> 269.9.
+// Same box, against the strip kernel: C4 x 32 284.6 -> 273.2 us (5.40 TB/s of planes in and depth out), x 8 79.0 -> 74.3, C2 x 80 290.7 -> 271.9.
 // Counters: one 32-bit word per queue, 128 bytes apart (p.sq_counters); a launch draws exactly K_q + W_q tickets from counter q (K_q
 // items, one failing ticket per wave: a wave draws only while the ticket before was good), and the wave that drew the last one puts the
 // counter back to zero when it ends: every launch starts from zero, the host zeroes the words once when it allocates them and after a
@@ -1541,7 +1538,7 @@ __global__ __launch_bounds__(256) void slx_stream_kernel(const SlxKParams p)
 //     chunks: drawn behind the wait for G(r), it is used when the row's arithmetic is done, at the end of the step;
 //   * items of ONE row (slx_plan.cpp): REF x 32 164.3 us with 1-row items, 171.3 with 2, 177.6 with 3, 192 with 8 -- the waves of a
 //     SIMD wait for their DMA here, and the more often they draw tickets the less they move in step.
-// Same-box A/B against the strip kernel: REF x 32 168.9 -> 166.1 us (-1.7 %), x 8 49.1 -> 48.1 (-2.0 %).  hipcc places the waits of the table
+// Same-box A/B against the strip kernel: REF x 32 169.7 -> 166.6 us (-1.8 %), x 8 49.2 -> 48.2 (-2.0 %).  hipcc places the waits of the table
 // look-up (codes other than the reflected one) behind the join of both arms: the DMA in flight is drained there in either case.  55.7 M vector instructions per launch for 59.9 M, the same bytes.  The Gray-MASK mode (x3: 62-quad spans with halo lanes)
 // was built on this kernel too, in five versions -- chip-wide queues (1 282 MB read for 885 algorithmic: the two waves that share a
 // halo line almost never share an L2), XCD-local queues (1 017 MB), one ticket per workgroup and item handed over through LDS (942 MB)

@@ -16,6 +16,7 @@ import pytest
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "structured-light-calculation_amd", "csrc")
 HIPCC = "/opt/rocm/bin/hipcc"
+NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]      # csrc/Makefile's
 
 MODE_GRAY_PHASE, MODE_MULTIFREQ, MODE_MULTIFREQ_GRAYMASK = 2, 3, 4
 
@@ -27,7 +28,7 @@ def kernels(tmp_path_factory):
         pytest.skip("hipcc is not installed")
     out = str(tmp_path_factory.mktemp("asm") / "slx_kernels.s")
     # the flags of csrc/Makefile
-    subprocess.check_call([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-I" + os.path.join(ROOT, "include"),
+    subprocess.check_call([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", *NO_PACKED, "-I" + os.path.join(ROOT, "include"),
                            "-I" + CSRC, "-S", "--cuda-device-only", os.path.join(CSRC, "slx_kernels.hip"), "-o", out],
                           stderr=subprocess.DEVNULL)
     text = open(out).read()
@@ -185,7 +186,7 @@ def test_stream_kernel_ticket_register_is_untouched_between_issue_and_wait(tmp_p
     if not os.path.exists(HIPCC):
         pytest.skip("hipcc is not installed")
     out = str(tmp_path / "slx_kernels.s")
-    subprocess.check_call([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-I" + os.path.join(ROOT, "include"),
+    subprocess.check_call([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", *NO_PACKED, "-I" + os.path.join(ROOT, "include"),
                            "-I" + CSRC, "-S", "--cuda-device-only", os.path.join(CSRC, "slx_kernels.hip"), "-o", out], stderr=subprocess.DEVNULL)
     lines = open(out).read().split("\n")
     NZ = 2
@@ -245,7 +246,7 @@ def test_fused_cloud_kernel_registers_match_the_plan(tmp_path):
     if not os.path.exists(HIPCC):
         pytest.skip("hipcc is not installed")
     out = str(tmp_path / "slx_cloud.s")
-    subprocess.check_call([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-I" + os.path.join(ROOT, "include"),
+    subprocess.check_call([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", *NO_PACKED, "-I" + os.path.join(ROOT, "include"),
                            "-I" + CSRC, "-S", "--cuda-device-only", os.path.join(CSRC, "slx_cloud.hip"), "-o", out], stderr=subprocess.DEVNULL)
     text = open(out).read()
     meta = text[text.index("amdhsa.kernels:"):]
@@ -270,7 +271,7 @@ def test_tracker_kernel_keeps_a_whole_frame_resident(tmp_path):
     if not os.path.exists(HIPCC):
         pytest.skip("hipcc is not installed")
     out = str(tmp_path / "slx_track.s")
-    subprocess.check_call([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-I" + os.path.join(ROOT, "include"),
+    subprocess.check_call([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", *NO_PACKED, "-I" + os.path.join(ROOT, "include"),
                            "-I" + CSRC, "-S", "--cuda-device-only", os.path.join(CSRC, "slx_track.hip"), "-o", out], stderr=subprocess.DEVNULL)
     text = open(out).read()
     meta = text[text.index("amdhsa.kernels:"):]

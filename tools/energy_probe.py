@@ -12,7 +12,7 @@ from bench import smi_sample          # noqa: E402  (one reader of rocm-smi for 
 
 EXE = os.path.join(ROOT, "tools", "energybench")
 if not os.path.exists(EXE):
-    subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", os.path.join(ROOT, "tools", "energybench.hip"), "-o", EXE])
+    subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", os.path.join(ROOT, "tools", "energybench.hip"), "-o", EXE])
 args = sys.argv[1:]
 seconds = float(args.pop(0)) if args and args[0].replace(".", "").isdigit() else 4.0
 classes = args or subprocess.run([EXE], capture_output=True, text=True).stdout.split("classes:")[1].split()

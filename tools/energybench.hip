@@ -2,7 +2,7 @@
 // while this program keeps one instruction class issuing on every SIMD).  The decode kernels of the Gray-free 4-step class hold
 // the card at its 1400 W cap (tools/power_probe.py): their launch time is energy / 1400 W, so the price list that matters for
 // them is joules per instruction, not cycles (tools/valubench.hip has those).
-//   hipcc --offload-arch=gfx950 -O3 tools/energybench.hip -o tools/energybench
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/energybench.hip -o tools/energybench
 //   tools/energybench CLASS SECONDS [WAVES_PER_SIMD]   -> one JSON line: wave-instructions per second, chip-wide
 // Each wave runs ITER x 8 independent instances of the instruction; operands are chosen so that values stay finite and differ
 // from lane to lane and from instance to instance (consecutive operations through an ALU see unrelated operands; whether that
@@ -47,9 +47,6 @@ constexpr int ITER = 16384;
 #define I_FMA32(k) "v_fma_f32 %" #k ", %" #k ", %8, %9\n"
 #define I_MUL32(k) "v_mul_f32 %" #k ", %" #k ", %8\n"
 #define I_ADD32(k) "v_add_f32 %" #k ", %" #k ", %9\n"
-#define I_PKFMA(k) "v_pk_fma_f32 %" #k ", %" #k ", %8, %9\n"
-#define I_PKMUL(k) "v_pk_mul_f32 %" #k ", %" #k ", %8\n"
-#define I_PKADD(k) "v_pk_add_f32 %" #k ", %" #k ", %9\n"
 #define I_FMA64(k) "v_fma_f64 %" #k ", %" #k ", %8, %9\n"
 #define I_MUL64(k) "v_mul_f64 %" #k ", %" #k ", %8\n"
 #define I_ADD64(k) "v_add_f64 %" #k ", %" #k ", %9\n"
@@ -66,27 +63,6 @@ constexpr int ITER = 16384;
 #define I_XOR(k) "v_xor_b32 %" #k ", %" #k ", %9\n"
 #define I_NOP(k) "s_nop 3\n"
 
-// the pk classes run on a 64-bit register pair: TYPE = double only names the register class, the halves are two floats
-// (1 + small, built from the double's bit pattern would be meaningless) -- so they get their own kernel with float2 operands
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-#define KERNEL_PK(NAME, INS, BEXPR, CEXPR)                                                            \
-    __global__ __launch_bounds__(256) void NAME(double *out, int iters)                              \
-    {                                                                                                 \
-        typedef float TYPE;                                                                           \
-        const float lane = (float)(threadIdx.x & 63u), wave = (float)(blockIdx.x & 7u);               \
-        f32x2 a[8];                                                                                   \
-        const float b1 = (BEXPR), c1 = (CEXPR);                                                       \
-        f32x2 b = {b1, b1 * 1.03125f}, c = {c1, c1 * 0.96875f};                                       \
-        for (int k = 0; k < 8; k++) {                                                                 \
-            const float v = 1.f + (lane * 8.f + (float)k) * (1.f / 520.f) + wave * (1.f / 16384.f);   \
-            a[k] = f32x2{v, 3.f - v};                                                                 \
-        }                                                                                             \
-        for (int i = 0; i < iters; i += 8) { BODY8(INS) BODY8(INS) BODY8(INS) BODY8(INS) BODY8(INS) BODY8(INS) BODY8(INS) BODY8(INS) }   \
-        float s = 0;                                                                                  \
-        for (int k = 0; k < 8; k++) s += a[k].x + a[k].y;                                             \
-        if (s == 12345.f) out[0] = s;                                                                 \
-    }
-
 KERNEL(k_fma32, float, I_FMA32, B_CONTRACT, C_UNIT)
 KERNEL(k_mul32, float, I_MUL32, B_NEARONE, C_UNIT)
 KERNEL(k_add32, float, I_ADD32, B_CONTRACT, C_SMALL)
@@ -94,9 +70,6 @@ KERNEL(k_add32, float, I_ADD32, B_CONTRACT, C_SMALL)
 // tools/valubench's loop did, and why its table showed plain multiplies / adds at half the cycles they take on finite data
 KERNEL(k_mul32_inf, float, I_MUL32, ((TYPE)1.5), C_UNIT)
 KERNEL(k_add32_inf, float, I_ADD32, B_CONTRACT, ((TYPE)3.0e38f))
-KERNEL_PK(k_pkfma, I_PKFMA, B_CONTRACT, C_UNIT)
-KERNEL_PK(k_pkmul, I_PKMUL, B_NEARONE, C_UNIT)
-KERNEL_PK(k_pkadd, I_PKADD, B_CONTRACT, C_SMALL)
 KERNEL(k_fma64, double, I_FMA64, B_CONTRACT, C_UNIT)
 KERNEL(k_mul64, double, I_MUL64, B_NEARONE, C_UNIT)
 KERNEL(k_add64, double, I_ADD64, B_CONTRACT, C_SMALL)
@@ -158,7 +131,6 @@ static const Entry kTable[] = {
     ENTRY("s_nop", float, k_nop),           ENTRY("v_mov_b32", float, k_mov32),     ENTRY("v_xor_b32", float, k_xor),
     ENTRY("v_mul_f32", float, k_mul32),     ENTRY("v_add_f32", float, k_add32),     ENTRY("v_fma_f32", float, k_fma32),
     ENTRY("v_mul_f32_inf", float, k_mul32_inf), ENTRY("v_add_f32_inf", float, k_add32_inf),
-    ENTRY("v_pk_mul_f32", double, k_pkmul), ENTRY("v_pk_add_f32", double, k_pkadd), ENTRY("v_pk_fma_f32", double, k_pkfma),
     ENTRY("v_sub_f32_sdwa", float, k_subsdwa), ENTRY("v_max3_f32", float, k_max3),  ENTRY("v_min_f32", float, k_min32),
     ENTRY("v_cmp_lt_f32", float, k_cmp32),  ENTRY("v_cndmask_b32", float, k_cndmask), ENTRY("v_rcp_f32", float, k_rcp32),
     ENTRY("v_mul_f64", double, k_mul64),    ENTRY("v_add_f64", double, k_add64),    ENTRY("v_fma_f64", double, k_fma64),

@@ -1,6 +1,6 @@
 // Micro-benchmark of the memory access patterns the decode kernel could use (GPU box only):
 // 12 u8 input planes read once, one f64 plane written once, 32 frame-sets of 1920x1200, no arithmetic.
-//   hipcc --offload-arch=gfx950 -O3 tools/membench.hip -o /tmp/membench && /tmp/membench
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/membench.hip -o /tmp/membench && /tmp/membench
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>

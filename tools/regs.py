@@ -4,7 +4,7 @@ import os, re, subprocess, sys
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 src = os.path.join(ROOT, "structured-light-calculation_amd", "csrc")
 out = "/tmp/slx_kernels_regs.s"
-subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-I" + os.path.join(ROOT, "include"),
+subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-I" + os.path.join(ROOT, "include"),
                        "-I" + src, "-S", "--cuda-device-only", os.path.join(src, "slx_kernels.hip"), "-o", out], stderr=subprocess.DEVNULL)
 s = open(out).read()
 only = sys.argv[1:] 

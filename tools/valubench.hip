@@ -1,7 +1,7 @@
 // Micro-benchmark of VALU issue cost per instruction type on gfx950 (GPU box only).
 // Every SIMD gets WAVES waves; each wave runs ITER x 8 independent instances of one instruction.
 // Prints the time per wave-instruction per SIMD relative to v_fma_f32.
-//   hipcc --offload-arch=gfx950 -O3 tools/valubench.hip -o tools/valubench && tools/valubench
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/valubench.hip -o tools/valubench && tools/valubench
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>
@@ -27,9 +27,6 @@ constexpr int ITER = 32768;
     }
 
 #define I_FMA32(k) "v_fma_f32 %" #k ", %" #k ", %8, %9\n"
-#define I_PKFMA(k) "v_pk_fma_f32 %" #k ", %" #k ", %8, %9\n"
-#define I_PKMUL(k) "v_pk_mul_f32 %" #k ", %" #k ", %8\n"
-#define I_PKADD(k) "v_pk_add_f32 %" #k ", %" #k ", %8\n"
 #define I_FMA64(k) "v_fma_f64 %" #k ", %" #k ", %8, %9\n"
 #define I_ADD64(k) "v_add_f64 %" #k ", %" #k ", %8\n"
 #define I_MUL64(k) "v_mul_f64 %" #k ", %" #k ", %8\n"
@@ -82,7 +79,6 @@ constexpr int ITER = 32768;
 #define I_BFI(k) "v_bfi_b32 %" #k ", %" #k ", %8, %9\n"
 #define I_LSHR(k) "v_lshrrev_b32 %" #k ", 8, %" #k "\n"
 #define I_ANDOR(k) "v_and_or_b32 %" #k ", %" #k ", %8, %9\n"
-#define I_PKMULBC(k) "v_pk_mul_f32 %" #k ", %8, %9\n"
 #define I_SUBSDWABC(k) "v_sub_f32_sdwa %" #k ", %8, %9 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1 src1_sel:BYTE_1\n"
 #define I_MULBC(k) "v_mul_f32 %" #k ", %8, %9\n"
 // b, c taken from the kernel argument bit for bit: denormal or normal operands on demand
@@ -96,7 +92,6 @@ constexpr int ITER = 32768;
         for (int k = 0; k < 8; k++) s += a[k];                                \
         if (s == (TYPE)12345) out[0] = s;                                     \
     }
-KERNEL_BC(k_pkmul_bc, double, I_PKMULBC)
 KERNEL_BC(k_subsdwa_bc, float, I_SUBSDWABC)
 KERNEL_BC(k_mul_bc, float, I_MULBC)
 KERNEL(k_cndv3, float, I_CNDV3)
@@ -143,9 +138,6 @@ KERNEL(k_cvtub, float, I_CVTUB)
 KERNEL(k_sdwa, float, I_SDWA)
 KERNEL(k_cndmask, float, I_CNDMASK)
 KERNEL(k_cmp32, float, I_CMP32)
-KERNEL(k_pkfma, double, I_PKFMA)
-KERNEL(k_pkmul, double, I_PKMUL)
-KERNEL(k_pkadd, double, I_PKADD)
 KERNEL(k_fma64, double, I_FMA64)
 KERNEL(k_add64, double, I_ADD64)
 KERNEL(k_mul64, double, I_MUL64)
@@ -281,15 +273,12 @@ static int run_bc(const char *name, void (*fn)(T *, T, T), T b, T c, double &bas
 }
 
 static float f_bits(uint32_t u) { float f; __builtin_memcpy(&f, &u, 4); return f; }
-static double d_bits(uint32_t lo, uint32_t hi) { uint64_t u = ((uint64_t)hi << 32) | lo; double d; __builtin_memcpy(&d, &u, 8); return d; }
 
 int main()
 {
     for (int w : {4}) {
         double base = 0;
         run("fma_f32", k_fma32, base, w);
-        run_bc("pkmul_norm", k_pkmul_bc, d_bits(0x40400000u, 0x40400000u), d_bits(0x7e800000u, 0x3f000000u), base, w);
-        run_bc("pkmul_denorm", k_pkmul_bc, d_bits(0x00000037u, 0x80000091u), d_bits(0x7e800000u, 0x7e800000u), base, w);
         run_bc("mul_norm", k_mul_bc, f_bits(0x40400000u), f_bits(0x7e800000u), base, w);
         run_bc("mul_denorm", k_mul_bc, f_bits(0x00000037u), f_bits(0x7e800000u), base, w);
         run_bc("subsdwa_bytes", k_subsdwa_bc, f_bits(0x00003700u), f_bits(0x00009100u), base, w);
@@ -336,9 +325,6 @@ int main()
         run("cvt_f32_ub", k_cvtub, base, w);
         run("sub_sdwa", k_sdwa, base, w);
         run("rcp_f32", k_rcp32, base, w);
-        run("pk_fma_f32", k_pkfma, base, w);
-        run("pk_mul_f32", k_pkmul, base, w);
-        run("pk_add_f32", k_pkadd, base, w);
         run("fma_f64", k_fma64, base, w);
         run("add_f64", k_add64, base, w);
         run("mul_f64", k_mul64, base, w);
