@@ -73,7 +73,7 @@ enum slx_status {
     SLX_ERR_UNAVAILABLE = -8      /* output not produced by this mode / not enabled in aux_outputs */
 };
 
-/* What one decode computes.  Stage names follow SURVEY.md section 8(a). */
+/* What one decode computes.  Stages: a1 wrapped phase, a2 arctangent, a3 / a4 Gray code, a5 merge, a6 / a7 triangulation. */
 enum slx_mode {
     SLX_MODE_PHASE_ONLY = 0,          /* CDecodePhase alone: pix (f64)                      */
     SLX_MODE_GRAY_ONLY = 1,           /* CDecodeGray alone: gray (f64)                      */
@@ -161,7 +161,8 @@ int slx_set_frame(slx_ctx *ctx, int group, int idx, const uint8_t *data, size_t 
  * any launch) once the context has decoded a batch outside a capture (its counters are allocated then).  The getters
  * below (slx_get_output, slx_get_depth, slx_get_point_cloud*) know nothing of a graph's replays: after a captured decode the CALLER
  * synchronizes the replay stream before calling them -- they read the context's output planes as the last completed replay left them.
- * Worked example and timings: INTEGRATION.md, "A fixed sequence of decodes as a hipGraph". */
+ * Replays are work the context does not see: a replay must not run at the same time as another replay of a graph captured from the same
+ * context, or as the context's own launches -- captured batches share the context's queue counters. */
 int slx_decode(slx_ctx *ctx, void *stream);
 
 /* n_sets frame-sets resident in device memory, one launch.  Plane p of set s starts at
@@ -364,10 +365,10 @@ int slx_pipe_collect(slx_pipe *pipe, const double **host_result, const double **
 const char *slx_pipe_last_error(const slx_pipe *pipe);
 
 /* ---- multi-GPU: one process per GPU, the final depth-map gather over RCCL / xGMI -------------------------------------
- * The decode is pixel-independent, so ranks exchange nothing while computing (SURVEY.md section 8e); the only
+ * The decode is pixel-independent, so ranks exchange nothing while computing; the only
  * collective is the gather of the finished depth maps.  Rank r holds the rows [row0, row0+rows) of the frame-sets
  * [set0, set0+n_sets) of a batch whose full result is f64 [total_sets][height][width]: whole frame-sets (rows == height)
- * or a row tile of every frame-set (the split BASELINE.json's north_star words).  The gather reassembles [set][H][W]
+ * or a row tile of every frame-set.  The gather reassembles [set][H][W]
  * on `root` (or on every rank, root = -1): grouped ncclSend / ncclRecv, one message per (peer, frame-set) landing at
  * its row offset of that set, so the root's 7 xGMI links carry traffic at once and no staging copy or transpose follows.
  * The reference has no counterpart (single process); this is the drop-in for a host loop that spreads a batch over a node. */

@@ -2,6 +2,6 @@
 
 Layout: csrc/ (HIP kernels + C ABI + the C++ mirror of the reference's decoder
 classes), api.py (ctypes binding of include/slx.h), synth.py (synthetic fringe
-source and the BASELINE.json workload configurations), shard.py (frame-set /
+source and the workload configurations C1..C5, REF), shard.py (frame-set /
 row-tile partition across ranks and the RCCL depth-map gather).
 """

@@ -186,7 +186,7 @@ size_t out_planes(const slx_config &c, int which)
     return 1;
 }
 
-// x1 weights; must stay the same formula as the documented spec (DESIGN.md "x1").
+// x1 weights; must stay the same formula as the documented spec (wy_k = cos(2 pi k / N), wx_k = sin(2 pi k / N), scale = 2 / N).
 void nstep_weights(int n, float *wy, float *wx, float *scale)
 {
     const double pi = 3.1415926535897932384626433832795;
@@ -1376,7 +1376,7 @@ int slx_track_next_batch(slx_ctx *ctx, const uint8_t *images, size_t stride_byte
     return rc;
 }
 
-// ---- frame ingest pipeline ---------------------------------------------------------
+// ---- frame ingest pipeline ---------------------------------------------------------------------------------------
 // Three streams, one event per stage and slot:
 //   copy-in  (h2d stream):    hipMemcpyAsync pinned -> device input               -> ev_in
 //   decode   (compute stream): waits ev_in, slx_decode_batch on the slot's buffers  -> ev_dec

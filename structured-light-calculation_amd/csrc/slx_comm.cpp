@@ -1,6 +1,6 @@
 // slx_comm.cpp -- the one collective of the path: the gather of finished depth maps over RCCL / xGMI.
 //
-// The reference is a single process (no distributed backend); BASELINE.json's north_star spreads a
+// The reference is a single process without a distributed backend; this library spreads a
 // batch over the 8 GPUs of a node by row tile and gathers the depth maps at the end.  Every decode stage is
 // pixel-independent, so this file is the only place where ranks talk to each other.
 //

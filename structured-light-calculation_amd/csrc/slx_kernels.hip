@@ -10,7 +10,7 @@
 // Every 8-bit input plane is read once, the f64 depth map is written once, and nothing
 // else touches HBM.  All arithmetic that the reference states in float/double is done with
 // the same IEEE operations in the same order (no FMA contraction); the only shortcuts are
-// ones that are provably bit-identical (see DESIGN.md "Exactness") and are verified
+// ones that are provably bit-identical (argued where they stand) and are verified
 // exhaustively against the oracle by tests/test_gpu_parity.py.
 //
 // R/ = DynaFrame/DynaFrame/ of the reference repository.
@@ -25,7 +25,7 @@
 #pragma clang fp contract(off)
 
 // Timing diagnostics, never part of the product build (tools/build_exp.sh builds tmp_ab/libslx_exp<N>.so with -DSLX_EXP=N): they leave
-// VALU work out -- the results are WRONG -- to show what the strip kernel's memory skeleton alone takes (DESIGN.md section 7, round 4):
+// VALU work out -- the results are WRONG -- to show what the strip kernel's memory skeleton alone takes:
 //   4: no triangulation   8: no temporal unwrap   16: no angle evaluation
 #ifndef SLX_EXP
 #define SLX_EXP 0
@@ -86,7 +86,7 @@ __device__ __forceinline__ int byte_diff(uint32_t a, uint32_t b)
 
 // a1 + a2 for N == 4, all in f32, from s2 = I0 - I2 and c2 = I1 - I3 (twice the reference's
 // sinValue / cosValue; integers in [-255, 255] held in floats).
-// Identities used (each argued in DESIGN.md, each covered by the exhaustive 511x511 tests):
+// Identities used (each covered by the exhaustive 511x511 tests):
 //  * sinValue/cosValue enter cvFastArctan only through their signs and the ratio min/max, and
 //    (a/2)/(b/2) == a/b exactly, so the halving is dropped;
 //  * for integer 0 <= a <= b <= 255, b >= 1, RN(a/b) == fma(fma(-b,q0,a), r, q0) with
@@ -878,7 +878,7 @@ __global__ __launch_bounds__(256) void slx_strip_kernel(const SlxKParams p)
     // them back into one hoisted register per plane: 24 SGPRs in the Gray modes, which spilled into VGPR lanes and came back
     // through v_readlane every row).
     // The Gray planes that ride the ring have a descriptor of their own (base = Gray plane 0 of this frame-set): the two plane groups
-    // may then live anywhere in memory -- separate allocations more than 2 GiB apart included (round 4: bench.py's REF launch fell back
+    // may then live anywhere in memory -- separate allocations more than 2 GiB apart included (behind one shared descriptor bench.py's REF launch fell back
     // to ordinary Gray loads, 200 against 166 us, when the allocator happened to place its two tensors that far apart).
     const __amdgpu_buffer_rsrc_t grsrc =
         GB > 0 ? __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p.gray[0] + gset), 0, 0xFFFFFFFFu, 0x00020000) : rsrc;
@@ -1280,9 +1280,9 @@ struct TicketQueue {
 };
 
 // ------------------------------------------------------------------------------------------
-// Stream kernel (round 4): the 3 x 4-step class (Gray-free, depth only) with work handed out in ADDRESS ORDER to resident waves.
+// Stream kernel: the 3 x 4-step class (Gray-free, depth only) with work handed out in ADDRESS ORDER to resident waves.
 //
-// What round 4 measured: the strip kernel's launch is its memory skeleton plus a tenth of its VALU time,
+// What was measured before it was built: the strip kernel's launch is its memory skeleton plus a tenth of its VALU time,
 // and the skeleton is 13 % faster with 2-row items than with 16-row items -- the memory system likes the chip's accesses to
 // advance through ONE frame-set in order -- while the arithmetic needs long items, because what an item sets up (lane geometry
 // by integer division, the column terms of cC / cD, descriptors) costs a third of a row.  Here a wave sets that state up once per
@@ -1526,7 +1526,7 @@ __global__ __launch_bounds__(256) void slx_stream_kernel(const SlxKParams p)
 }
 
 // ------------------------------------------------------------------------------------------
-// Stream kernel of the reference's own mode (round 6): SLX_MODE_GRAY_PHASE -- a1 + a3 + a4 + a5 + a7, R/CCalculation.cpp:525-592 + :666-708,
+// Stream kernel of the reference's own mode: SLX_MODE_GRAY_PHASE -- a1 + a3 + a4 + a5 + a7, R/CCalculation.cpp:525-592 + :666-708,
 // 6 Gray bits whose 12 planes ride the DMA ring.  The strip kernel serves that mode with 3-row items -- the shortest-lived work items
 // of the library, so what an item sets up (lane geometry by integer division, the buffer descriptors, the column terms of cC / cD)
 // is paid every third row.  Here, as in slx_stream_kernel, a resident wave sets that up once per LAUNCH and takes R-row items of ONE
@@ -1771,7 +1771,7 @@ __global__ __launch_bounds__(256) void slx_gstream_kernel(const SlxKParams p)
 // The reference's decoder objects on the strip path: what CDecodePhase::Decode (R/CDecodePhase.cpp:83-96 -> CountResult :48-80:
 // four 8-bit planes in, the wrapped phase in projector pixels out as CV_64FC1) and CDecodeGray::Decode (R/CDecodeGray.cpp:108-139
 // -> Grey2Bin :150-176, CountResult :179-204: 2 G planes in, the stripe's left edge out as CV_64FC1) compute, for a host loop that
-// keeps the reference's two-decoder structure (INTEGRATION.md section 1) instead of the fused call.  Same work items, same
+// keeps the reference's two-decoder structure instead of the fused call.  Same work items, same
 // HBM -> LDS DMA ring (one chunk = a row of the decoder's planes, two chunks ahead, counted waits), same staged lane-contiguous
 // nontemporal stores as slx_strip_kernel above; the arithmetic is that kernel's wrapped_pix_from_diffs / SWAR Gray pack.
 //   MODE = SLX_MODE_PHASE_ONLY: 4 planes (the reference's 4 steps), 4 + 8 = 12 B/px

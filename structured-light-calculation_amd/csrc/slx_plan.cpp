@@ -1,7 +1,7 @@
 // slx_plan.cpp -- host-side planning of a decode launch: which kernel, how the frame-sets are cut into work items, the grid.
 //
 // Nothing here touches the GPU or the HIP runtime: the same translation unit is compiled into libslx.so and, by g++ with
-// -fsanitize=address,undefined, into tests/cpp/host_sanitize (SURVEY.md section 5: sanitizers on the CPU side), which walks
+// -fsanitize=address,undefined, into tests/cpp/host_sanitize (sanitizers on the CPU side), which walks
 // many tile shapes through slx_plan_launch and checks that the items of every plan cover every row of every frame-set
 // exactly once and that no 32-bit offset the kernel forms can wrap.  slx_kernels.hip holds the kernels and launches a plan.
 #include <algorithm>
@@ -223,7 +223,7 @@ int slx_plan_launch(const SlxKParams &kp_in, int mode, bool aux, int n_sets, int
     while (h) { const unsigned r = g % h; g = h; h = r; }          // gcd(QR, 64)
     kp.interleave = 64u / g;
     // Weave: more rows per row group than whole waves need -- a lane's rows are then `interleave` apart and the waves of a group
-    // sweep that many consecutive rows in step.  Measured (tools/ab.py, round 4, two boxes): 8 rows instead of 2 on the 1920-wide
+    // sweep that many consecutive rows in step.  Measured (tools/ab.py, two boxes): 8 rows instead of 2 on the 1920-wide
     // 4-step kernels, config 4 282.9 -> 277.1 us (-2.0 %; the other box 290.1 -> 285.8), config 3 215.5 -> 209.9 (-2.6 %); 16 rows
     // lose it again; the 1280-wide cases (one row = 5 whole chunks) lose 0.5-1.7 % with any weave and are left alone, 4096-wide
     // 8-step within noise.  Only full frames: a row group of 8 x rows-per-item rows wastes too much of a short tile.
@@ -247,7 +247,7 @@ int slx_plan_launch(const SlxKParams &kp_in, int mode, bool aux, int n_sets, int
         if (kp.gray_step < 256u) kp.dma_imm = 0;
     }
     // Stream kernel (slx_kernels.hip: slx_stream_kernel): the Gray-free 4-step depth-only class, launches that fill the chip many times over.
-    // (An instantiation with the optional planes x, y, U, k was built and measured in round 5 -- C4 x 8 / 16 / 32 frame-sets: +1.5 / -1.6 /
+    // (An instantiation with the optional planes x, y, U, k was built and measured -- C4 x 8 / 16 / 32 frame-sets: +1.5 / -1.6 /
     // -0.6 % against the strip kernel on the same box -- and is not in the tree.)
     plan->stream = 0;
     if (!decoder && mode == SLX_MODE_MULTIFREQ && kp.n_steps == 4 && kp.dma_imm && !aux && kp.sq_counters && tn.stream != 1 && tn.weave <= 1) {
@@ -267,9 +267,8 @@ int slx_plan_launch(const SlxKParams &kp_in, int mode, bool aux, int n_sets, int
         // as many queues as the launch has waves (a partitioned or small device: fewer than 255 resident waves), else a queue's row
         // groups would never be decoded
         const unsigned m = cpg <= 255u ? (unsigned)std::min<unsigned long long>(255u / cpg, waves / cpg) : 0u;
-        // >= 5 items per resident wave.  Same-box sweep of round 5 (tools/stream_sweep.sh, C4 x 4 ... 31 frame-sets, stream against strip
-        // kernel): 4 sets -3 % (the minima equal), 6 sets -6 %, 8 -10 %, 10 -14 %, 12 -10 %, 16 -7 %, 20 ... 24 -6 %, 28 ... 31 -3 %: the
-        // queues pay from about 5 items per wave on (round 4's threshold was 8)
+        // >= 5 items per resident wave.  Same-box sweep (C4 x 4 ... 31 frame-sets, stream against strip kernel): 4 sets +3 %, 5 -4 %, 6 -5 %,
+        // 8 -7 %, 10 -5 %, 16 -4 %, 24 -4 %, 31 -3 %; C2 x 20 -6 %, 32 -5 %, 80 -5 %: the queues pay from about 5 items per wave on
         const bool big = groups_total * cpg >= 5ull * waves;
         if (m >= 1 && cpg * m <= SLX_STREAM_MAX_QUEUES && groups_total * gps < (1ull << 32) && groups_total < (1ull << 31) &&
             (tn.stream == 2 ? groups_total * cpg >= 1 : big)) {
@@ -295,10 +294,10 @@ int slx_plan_launch(const SlxKParams &kp_in, int mode, bool aux, int n_sets, int
             return 0;
         }
     }
-    // Stream kernel of the reference's own mode (slx_gstream_kernel, round 6): 6 Gray bits on the ring + one 4-step frequency, depth only.
+    // Stream kernel of the reference's own mode (slx_gstream_kernel): 6 Gray bits on the ring + one 4-step frequency, depth only.
     // Same queues and counters as slx_stream_kernel; a row is two ring chunks there, an item ONE row (REF x 32: 164.3 us with 1-row
     // items, 171.3 with 2, 177.6 with 3: profiles/r06_gstream_ab.log).  Taken from 8 items per resident wave on -- same-box against the
-    // strip kernel: 32 frame-sets of the reference's size -3.1 %, 16 -3.5 %, 8 -2.4 %, 4 (5 items per wave) +0.7 %.
+    // strip kernel: 32 frame-sets of the reference's size -1.9 %, 16 -2.9 %, 8 -3.8 %, 7 -3.3 %.
     if (!decoder && gb == 6 && mode == SLX_MODE_GRAY_PHASE && kp.n_steps == 4 && kp.dma_imm && !aux && kp.sq_counters && tn.stream != 1 && tn.weave <= 1) {
         const unsigned il = 64u / g, cpg = il * QR / 64u;
         const unsigned R = (tn.stream_rows >= 1 && tn.stream_rows <= 16) ? (unsigned)tn.stream_rows : 1u;

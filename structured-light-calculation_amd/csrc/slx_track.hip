@@ -1,4 +1,4 @@
-// slx_track.hip -- the dynamic-frame tracker of DynaFrame for gfx950 (SURVEY.md section 8f, rank 3).
+// slx_track.hip -- the dynamic-frame tracker of DynaFrame for gfx950.
 //
 //   CCalculation::StripRegression      R/CCalculation.cpp:789-892  -> slx_strip_regression_kernel
 //   CCalculation::FillOtherDeltaProU   R/CCalculation.cpp:595-663  -> slx_delta_p_kernel + slx_track_update_kernel
@@ -200,7 +200,7 @@ __global__ __launch_bounds__(256) void slx_track_update_kernel(const float *raw,
 // HBM: a workgroup computes it for its band of kFusedRows rows plus one halo row above and below and one halo column either
 // side (the strips of those halo pixels are computed a second time by the neighbouring workgroup: 25 % more scan work for
 // 8 bytes per pixel less traffic and one launch less), keeps it in LDS, and blurs from there.
-// Tile geometry (round 5): 254 of a workgroup's 256 lanes own an output column (the first and the last lane stand on the blur's halo
+// Tile geometry: 254 of a workgroup's 256 lanes own an output column (the first and the last lane stand on the blur's halo
 // columns and only scan).  The sliding sums cover the 2 HW = 20 columns the scan reaches beyond them as well, 276 in all, and are formed
 // TWO columns per lane by the first 138 lanes (16-bit loads, both columns in the halves of one register).  Before, the scan's reach
 // took 22 of every workgroup's lanes: 1920 columns were 9 tiles of 234, the ninth a fifth full, 1 350 workgroups for 256 CUs; now 8
@@ -235,7 +235,7 @@ __global__ __launch_bounds__(kTile) void slx_track_fused_kernel(const uint8_t *c
         p.stamps[4 * (size_t)blockIdx.x + 0] = __builtin_amdgcn_s_memtime();
         p.stamps[4 * (size_t)blockIdx.x + 2] = __builtin_amdgcn_s_memrealtime();
     }
-    // XCD-aware tile order (round 5).  The dispatcher deals workgroups round-robin over the 8 XCDs, each with its own L2; a band shares 22
+    // XCD-aware tile order.  The dispatcher deals workgroups round-robin over the 8 XCDs, each with its own L2; a band shares 22
     // of its 30 image rows and 2 of its 10 rows of the previous frame's strips with the bands above and below it, and in plain order
     // those neighbours sit on other XCDs: the shared rows came from HBM once per band (74.9 MB read per frame for 57.6 algorithmic,
     // profiles/r05_track_pmc_summary.json).  Here XCD x takes a contiguous run of tiles in row-major order, so that a tile's vertical

@@ -1,12 +1,11 @@
 """Partition of a batch of frame-sets across ranks, and the final depth-map gather.
 
-The decode itself is pixel-independent (SURVEY.md section 8e), so ranks never
+The decode itself is pixel-independent, so ranks never
 exchange data while computing; the only collective is the gather of finished
 depth maps (RCCL over xGMI on GPUs -- torch.distributed backend "nccl" -- or
 gloo on CPU in the tests).  Two ways to cut the work, both exact:
   * by frame-set: rank r decodes whole frame-sets [lo, hi);
-  * by row-tile:  rank r decodes rows [lo, hi) of every frame-set (the split
-    BASELINE.json's north_star words); the tile's row_offset keeps (v - cy) of
+  * by row-tile:  rank r decodes rows [lo, hi) of every frame-set; the tile's row_offset keeps (v - cy) of
     R/CCalculation.cpp:160 referring to the full-frame row.
 """
 import torch

@@ -59,7 +59,7 @@ def scaled_calibration(width, height, proj_width, trans_scale=10.0):
 
 
 def make_spec(name):
-    """Workload configurations of BASELINE.json (C1..C5) plus the reference's
+    """Workload configurations C1..C5 plus the reference's
     compiled-in case (REF: 1280x1024, 6-bit Gray + 4-step at T = 40)."""
     def base(w, h, pw, mode, periods, n_steps=4, gray_bits=0):
         spec = {
@@ -104,7 +104,7 @@ def n_planes(spec):
 
 
 def algorithmic_bytes_per_pixel(spec):
-    """each u8 input read once + one f64 depth written."""
+    """Each u8 input read once + one f64 depth written."""
     n_phase, n_gray = n_planes(spec)
     return n_phase + n_gray + 8
 
